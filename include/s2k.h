@@ -47,13 +47,14 @@ enum {
     S2K_ERR_NO_DEVICE = -8    /* no CUDA device visible */
 };
 
-/* ggml type ids accepted by s2k_model_upload_tensor */
+/* ggml type ids accepted by s2k_model_upload_tensor (BF16: operator tensors only) */
 enum {
     S2K_TYPE_F32 = 0,
     S2K_TYPE_F16 = 1,
     S2K_TYPE_Q8_0 = 8,
     S2K_TYPE_Q4_K = 12,
-    S2K_TYPE_Q6_K = 14
+    S2K_TYPE_Q6_K = 14,
+    S2K_TYPE_BF16 = 30
 };
 
 /* Mirrors s2::ModelHParams (include/s2_model.h:38-69) plus head_dim, which the
@@ -544,6 +545,98 @@ S2K_API s2k_status s2k_codec_stream_push(s2k_codec_stream *s, const int32_t *fra
 S2K_API s2k_status s2k_codec_stream_finish(s2k_codec_stream *s, float *pcm, size_t cap, int64_t *n_pcm);
 /* PCM samples the next push / finish can release at most (capacity to give). */
 S2K_API int64_t s2k_codec_stream_max_release(const s2k_codec_stream *s);
+
+/* ---- Operators on device memory (no reference counterpart: its cache is f16
+ * and its sampler works on host logits).  Every pointer below is device memory
+ * of the named device; work is enqueued on `stream` (a cudaStream_t of that
+ * device, NULL: its default stream) and the call returns without waiting.  The
+ * calls keep nothing: no workspace, no state between calls, so calls on
+ * different streams do not disturb each other, and every call may be captured
+ * into a CUDA graph.  The current device is left as it was.  Sizes and
+ * pointers are checked on the host before anything is enqueued. */
+
+/* A paged KV cache in 8 bits.  A page holds 16 tokens of every (layer, kv
+ * head); a value stands for its int8 (in [-127, 127]) times its block's scale,
+ * a block being one page of one layer and kv head.  k and v 16-byte aligned;
+ * head_dim 64 or 128. */
+typedef struct s2k_kv8 {
+    int8_t *k;      /* [n_pages][n_layers][n_kv_heads][16][head_dim] */
+    int8_t *v;      /* [n_pages][n_layers][n_kv_heads][head_dim][16]: transposed */
+    float *k_scale; /* [n_pages][n_layers][n_kv_heads] */
+    float *v_scale; /* [n_pages][n_layers][n_kv_heads] */
+    int32_t device, n_pages, n_layers, n_kv_heads, head_dim;
+} s2k_kv8;
+
+/* The rows of a call, as the tokens of n_seqs sequences: sequence b owns rows
+ * row_start[b] .. row_start[b+1] - 1 (row_start NULL: max_rows rows each),
+ * which sit at positions past[b], past[b] + 1, ...; its position p lives in
+ * page block_table[b][p / 16], slot p % 16.  past, row_start and block_table
+ * are read on the device when the call runs.  A sequence whose entries do not
+ * fit (a negative count or past, more than max_rows rows, rows beyond n_rows,
+ * positions beyond the table) is skipped, and so is a page that is none of the
+ * cache's; each sets bit 8 of *err where err is given.  Rows of no sequence
+ * are neither read nor written. */
+typedef struct s2k_kv8_rows {
+    int32_t n_seqs, n_rows;
+    int32_t max_rows;           /* most rows of one sequence */
+    int32_t table_ld;           /* entries per row of block_table */
+    const int32_t *past;        /* [n_seqs] positions held before this call's rows */
+    const int32_t *row_start;   /* [n_seqs + 1] or NULL */
+    const int32_t *block_table; /* [n_seqs][table_ld] */
+    int32_t *err;               /* optional device word */
+} s2k_kv8_rows;
+
+/* Rows of heads: element d of head h of row r is data[r * row_stride +
+ * h * head_stride + d] (strides in elements).  type: S2K_TYPE_F32, F16, BF16. */
+typedef struct s2k_heads {
+    void *data;
+    int64_t row_stride, head_stride;
+    int32_t type;
+} s2k_heads;
+
+/* Stores the rows' keys and values (same type) into the cache.  A block's
+ * scale is max|x| / 127 over its tokens, the values are x / scale rounded to
+ * the nearest integer (ties to even).  A page that already holds positions
+ * before past[b] keeps its scale unless a new token needs a larger one; what
+ * it holds is then rounded again under that.  A page entered at its first slot
+ * starts afresh.  A block with a NaN or an infinity reads as NaN from then on.
+ * A page that the call writes must belong to one sequence of the call. */
+S2K_API s2k_status s2k_kv8_append(const s2k_kv8 *c, int32_t layer, const s2k_kv8_rows *r, const s2k_heads *k,
+                                  const s2k_heads *v, void *stream);
+
+/* The keys and values that the rows' positions hold (value * scale), written
+ * to k and v (same type): the inverse of s2k_kv8_append up to its rounding. */
+S2K_API s2k_status s2k_kv8_read(const s2k_kv8 *c, int32_t layer, const s2k_kv8_rows *r, const s2k_heads *k,
+                                const s2k_heads *v, void *stream);
+
+/* Attention of the rows' queries over their sequences' cached positions, the
+ * rows' own (stored by s2k_kv8_append before) among them:
+ *   out = sum_j softmax_j(scale * q . k_j) v_j
+ * over the keys j <= p of the row's position p with window == 0, or
+ * j > p - window (the last `window` keys), or j < sinks (the first ones).
+ * n_heads query heads share the kv heads in groups of n_heads / n_kv_heads.
+ * q and out have the same type; out may be q.  Sums and softmax statistics
+ * are f32.  A row that sees no key (all its pages skipped) is zero. */
+S2K_API s2k_status s2k_kv8_attend(const s2k_kv8 *c, int32_t layer, const s2k_kv8_rows *r, const s2k_heads *q,
+                                  const s2k_heads *out, int32_t n_heads, float scale, int32_t window, int32_t sinks,
+                                  void *stream);
+
+/* Most alternatives of s2k_logprobs. */
+#define S2K_LOGPROBS_MAX_TOP 32
+
+/* Log probabilities under the softmax of each of `rows` rows of n logits
+ * (type F32, F16 or BF16, row_stride elements apart) on `device`:
+ *   logprob [rows]            of targets[row]; NaN where the target is outside [0, n)
+ *   entropy [rows]            in nats
+ *   top_ids, top_logprobs     [rows][n_top] the n_top (0..32, <= n) largest logits, largest
+ *                             first, ties to the lowest index
+ * logprob (with targets) and entropy may be NULL.  A logit of -inf is a masked
+ * token (probability 0); a row of only those has entropy 0 and log
+ * probabilities of -inf.  A row with a NaN or +inf has NaN in their place;
+ * its top_ids order NaN below every number. */
+S2K_API s2k_status s2k_logprobs(int32_t device, const void *logits, int32_t type, int32_t rows, int32_t n,
+                                int64_t row_stride, const int32_t *targets, int32_t n_top, float *logprob,
+                                float *entropy, int32_t *top_ids, float *top_logprobs, void *stream);
 
 #ifdef __cplusplus
 }

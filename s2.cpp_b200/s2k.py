@@ -46,6 +46,7 @@ EXPORTED = [
     "s2k_codec_receptive_frames", "s2k_codec_decode", "s2k_codec_decode_range", "s2k_codec_decode_windowed",
     "s2k_codec_stream_create", "s2k_codec_stream_free", "s2k_codec_stream_push", "s2k_codec_stream_finish",
     "s2k_codec_stream_max_release",
+    "s2k_kv8_append", "s2k_kv8_read", "s2k_kv8_attend", "s2k_logprobs",
 ]
 
 REQ_WAITING, REQ_LIVE, REQ_DONE, REQ_FAILED, REQ_CANCELLED = 0, 1, 2, 3, 4  # S2K_REQ_*
@@ -106,6 +107,26 @@ class _CodecHParams(ctypes.Structure):
                 ("rvq_block_size", ctypes.c_int32), ("rvq_n_layer", ctypes.c_int32),
                 ("rvq_n_local_heads", ctypes.c_int32), ("rvq_head_dim", ctypes.c_int32), ("rvq_dim", ctypes.c_int32),
                 ("rvq_rope_base", ctypes.c_float), ("rvq_norm_eps", ctypes.c_float)]
+
+
+class _KV8(ctypes.Structure):
+    """s2k_kv8"""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("device", ctypes.c_int32), ("n_pages", ctypes.c_int32),
+                ("n_layers", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+class _KV8Rows(ctypes.Structure):
+    """s2k_kv8_rows"""
+    _fields_ = [("n_seqs", ctypes.c_int32), ("n_rows", ctypes.c_int32), ("max_rows", ctypes.c_int32),
+                ("table_ld", ctypes.c_int32), ("past", ctypes.c_void_p), ("row_start", ctypes.c_void_p),
+                ("block_table", ctypes.c_void_p), ("err", ctypes.c_void_p)]
+
+
+class _Heads(ctypes.Structure):
+    """s2k_heads"""
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("type", ctypes.c_int32)]
 
 
 def codec_hp_struct(ch, cls=_CodecHParams):
@@ -224,6 +245,10 @@ def lib() -> ctypes.CDLL:
         "s2k_codec_stream_push": ([vp, vp, vp, ctypes.c_size_t, i64p], i32),
         "s2k_codec_stream_finish": ([vp, vp, ctypes.c_size_t, i64p], i32),
         "s2k_codec_stream_max_release": ([vp], ctypes.c_int64),
+        "s2k_kv8_append": ([vp, i32, vp, vp, vp, vp], i32),
+        "s2k_kv8_read": ([vp, i32, vp, vp, vp, vp], i32),
+        "s2k_kv8_attend": ([vp, i32, vp, vp, vp, i32, ctypes.c_float, i32, i32, vp], i32),
+        "s2k_logprobs": ([i32, vp, i32, i32, i32, ctypes.c_int64, vp, i32, vp, vp, vp, vp, vp], i32),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name)
@@ -845,3 +870,174 @@ class CodecStream:
             self.close()
         except Exception:
             pass
+
+
+# --- operators on device memory: torch CUDA tensors in and out, on the current stream ---
+
+_OP_TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 30}  # S2K_TYPE_F32 / F16 / BF16
+_op_type_of = {}  # torch dtype -> S2K_TYPE_*
+
+
+def _op_type(what: str, t) -> int:
+    code = _op_type_of.get(t.dtype)
+    if code is None:
+        code = _OP_TYPES.get(str(t.dtype))
+        if code is None:
+            raise S2KError(-7, f"{what} has type {t.dtype} (float32, float16 or bfloat16)")
+        _op_type_of[t.dtype] = code
+    return code
+
+
+def _op_stream(device: int, stream) -> int:
+    if stream is None:
+        import torch
+        return torch.cuda.current_stream(device).cuda_stream
+    return int(getattr(stream, "cuda_stream", stream))
+
+
+def _on_device(what: str, t, device: int) -> int:
+    """Data pointer of a CUDA tensor of `device`."""
+    if t.get_device() != device:
+        raise S2KError(-1, f"{what} is not on CUDA device {device}")
+    return t.data_ptr()
+
+
+def _ints(what: str, t, shape, device: int) -> int:
+    """Data pointer of a contiguous int32 tensor."""
+    if str(t.dtype) != "torch.int32" or tuple(t.shape) != shape or not t.is_contiguous():
+        raise S2KError(-1, f"{what} must be a contiguous int32 tensor of shape {list(shape)}")
+    return _on_device(what, t, device)
+
+
+class KV8Cache:
+    """A paged KV cache in 8 bits over the caller's device memory (s2k_kv8):
+    pages of 16 tokens, int8 values, one f32 scale per (page, layer, kv head)
+    for the keys and one for the values.
+
+      k        int8 [pages][layers][kv_heads][16][head_dim]
+      v        int8 [pages][layers][kv_heads][head_dim][16]
+      k_scale, v_scale   float32 [pages][layers][kv_heads]
+
+    `append`, `read` and `attend` enqueue on the current torch stream of the
+    cache's device (or `stream`) and do not wait.  Their rows belong to
+    sequences: past [n_seqs] positions held before the call, block_table
+    [n_seqs][entries] page numbers, row_start [n_seqs + 1] first row of each
+    sequence (None: the rows are shared out evenly), max_rows the most rows of
+    one sequence.  These three are int32 CUDA tensors that the kernels read.  An
+    optional int32 tensor `err` gets bit 8 set where an entry does not fit (see
+    s2k_kv8_rows); such rows, and rows of no sequence, are left unwritten."""
+
+    PAGE = 16
+
+    def __init__(self, k, v, k_scale, v_scale):
+        if k.dim() != 5 or k.shape[3] != 16:
+            raise S2KError(-1, "k must be int8 [pages][layers][kv_heads][16][head_dim]")
+        P, L, H, _, D = k.shape
+        self.device = k.get_device()
+        for what, t, dtype, shape in (("k", k, "torch.int8", (P, L, H, 16, D)), ("v", v, "torch.int8", (P, L, H, D, 16)),
+                                      ("k_scale", k_scale, "torch.float32", (P, L, H)),
+                                      ("v_scale", v_scale, "torch.float32", (P, L, H))):
+            if str(t.dtype) != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+                raise S2KError(-1, f"{what} must be a contiguous {dtype[6:]} tensor of shape {list(shape)}")
+            if self.device < 0 or t.get_device() != self.device:
+                raise S2KError(-1, f"{what} is not on the CUDA device of the cache")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_pages, self.n_layers, self.n_kv_heads, self.head_dim = P, L, H, D
+        self._c = _KV8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.device, P, L, H, D)
+
+    @classmethod
+    def empty(cls, n_pages: int, n_layers: int, n_kv_heads: int, head_dim: int, device: int = 0) -> "KV8Cache":
+        """A cache in memory of its own."""
+        import torch
+        shape, dev = (n_pages, n_layers, n_kv_heads), f"cuda:{device}"
+        return cls(torch.zeros(shape + (16, head_dim), dtype=torch.int8, device=dev),
+                   torch.zeros(shape + (head_dim, 16), dtype=torch.int8, device=dev),
+                   torch.zeros(shape, device=dev), torch.zeros(shape, device=dev))
+
+    def _rows(self, n_rows: int, past, block_table, row_start, max_rows, err) -> _KV8Rows:
+        dev, n = self.device, past.shape[0] if past.dim() == 1 else -1
+        if block_table.dim() != 2:
+            raise S2KError(-1, "block_table must be [n_seqs][entries]")
+        ld = block_table.shape[1]
+        if max_rows is None:
+            if row_start is not None or n <= 0 or n_rows % n:
+                raise S2KError(-1, "max_rows is needed where rows are not shared out evenly")
+            max_rows = n_rows // n
+        return _KV8Rows(n, n_rows, max_rows, ld, _ints("past", past, (n,), dev),
+                        None if row_start is None else _ints("row_start", row_start, (n + 1,), dev),
+                        _ints("block_table", block_table, (n, ld), dev),
+                        None if err is None else _ints("err", err, (1,), dev))
+
+    def _heads(self, what: str, t, n_heads) -> _Heads:
+        s = t.stride() if t.dim() != 3 or t.shape[0] else (t.shape[1] * t.shape[2], t.shape[2], 1)  # no rows: any
+        if len(s) != 3 or t.shape[2] != self.head_dim or (n_heads is not None and t.shape[1] != n_heads) or s[2] != 1:
+            raise S2KError(-1, f"{what} must be [rows][heads][{self.head_dim}] with a dense last dimension")
+        return _Heads(_on_device(what, t, self.device), s[0], s[1], _op_type(what, t))
+
+    def append(self, layer: int, k, v, past, block_table, row_start=None, max_rows: Optional[int] = None, err=None,
+               stream=None) -> None:
+        """Stores rows [rows][kv_heads][head_dim] of keys and values (s2k_kv8_append)."""
+        if k.shape != v.shape:
+            raise S2KError(-1, "k and v have different shapes")
+        r = self._rows(k.shape[0], past, block_table, row_start, max_rows, err)
+        kh, vh = self._heads("k", k, self.n_kv_heads), self._heads("v", v, self.n_kv_heads)
+        _check(lib().s2k_kv8_append(ctypes.byref(self._c), layer, ctypes.byref(r), ctypes.byref(kh), ctypes.byref(vh),
+                                    _op_stream(self.device, stream)))
+
+    def read(self, layer: int, n_rows: int, past, block_table, row_start=None, max_rows: Optional[int] = None,
+             dtype=None, out=None, err=None, stream=None):
+        """(k, v) [n_rows][kv_heads][head_dim] that the rows' positions hold, float32 or `dtype`, or written to
+        the pair `out` (s2k_kv8_read)."""
+        if out is None:
+            shape = (n_rows, self.n_kv_heads, self.head_dim)
+            dtype = self.k_scale.dtype if dtype is None else dtype
+            out = (self.k_scale.new_empty(shape, dtype=dtype), self.k_scale.new_empty(shape, dtype=dtype))
+        if out[0].shape[0] != n_rows or out[1].shape[0] != n_rows:
+            raise S2KError(-1, f"out must hold {n_rows} rows")
+        r = self._rows(n_rows, past, block_table, row_start, max_rows, err)
+        kh, vh = self._heads("k", out[0], self.n_kv_heads), self._heads("v", out[1], self.n_kv_heads)
+        _check(lib().s2k_kv8_read(ctypes.byref(self._c), layer, ctypes.byref(r), ctypes.byref(kh), ctypes.byref(vh),
+                                  _op_stream(self.device, stream)))
+        return out[0], out[1]
+
+    def attend(self, layer: int, q, past, block_table, row_start=None, max_rows: Optional[int] = None,
+               scale: Optional[float] = None, window: int = 0, sinks: int = 0, out=None, err=None, stream=None):
+        """Attention of rows q [rows][heads][head_dim] over their sequences' cached positions, causal, with the
+        last `window` keys (0: all) and the first `sinks` keys visible (s2k_kv8_attend); scale defaults to
+        head_dim ** -0.5.  Returns out, a tensor like q unless given."""
+        if out is None:
+            out = q.new_empty(q.shape)
+        if out.shape != q.shape:
+            raise S2KError(-1, "q and out have different shapes")
+        r = self._rows(q.shape[0], past, block_table, row_start, max_rows, err)
+        qh, oh = self._heads("q", q, None), self._heads("out", out, None)
+        if scale is None:
+            scale = self.head_dim ** -0.5
+        _check(lib().s2k_kv8_attend(ctypes.byref(self._c), layer, ctypes.byref(r), ctypes.byref(qh), ctypes.byref(oh),
+                                    q.shape[1], scale, window, sinks, _op_stream(self.device, stream)))
+        return out
+
+
+def logprobs(logits, targets=None, n_top: int = 0, stream=None):
+    """(logprob [rows], entropy [rows], top_ids [rows][n_top], top_logprobs [rows][n_top]) of logits [rows][n]
+    (s2k_logprobs): the log probability of each row's target (int32 CUDA tensor [rows]; None without targets), the
+    entropy in nats, and the n_top (<= 32) most likely tokens, ties to the lowest index (both None for n_top 0)."""
+    if logits.dim() != 2 or logits.shape[1] == 0 or (logits.shape[0] and logits.stride(1) != 1):
+        raise S2KError(-1, "logits must be [rows][n] with a dense last dimension")
+    import torch
+    rows, n = logits.shape
+    dev, code = logits.get_device(), _op_type("logits", logits)
+    x = _on_device("logits", logits, dev) if dev >= 0 else None
+    if x is None:
+        raise S2KError(-1, "logits is not on a CUDA device")
+    tgt = None if targets is None else _ints("targets", targets, (rows,), dev)
+    res = logits.new_empty((2, rows), dtype=torch.float32)
+    ids = top = None
+    if n_top > 0:
+        ids = logits.new_empty((rows, n_top), dtype=torch.int32)
+        top = logits.new_empty((rows, n_top), dtype=torch.float32)
+    _check(lib().s2k_logprobs(dev, x, code, rows, n, max(logits.stride(0), 0), tgt, n_top,
+                              None if tgt is None else res.data_ptr(), res.data_ptr() + 4 * rows,
+                              None if ids is None else ids.data_ptr(), None if top is None else top.data_ptr(),
+                              _op_stream(dev, stream)))
+    return (None if tgt is None else res[0]), res[1], ids, top
