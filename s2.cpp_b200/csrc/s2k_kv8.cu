@@ -170,19 +170,6 @@ __global__ void __launch_bounds__(kKv8Warps * 32) kv8_read_kernel(Kv8 c, Kv8Rows
     }
 }
 
-template <class F>
-static cudaError_t kv8_dispatch(int hd, int type, F f) {
-    switch (hd * 100 + type) {
-        case 12800 + OT_F32: return f(std::integral_constant<int, 128>(), std::integral_constant<int, OT_F32>());
-        case 12800 + OT_F16: return f(std::integral_constant<int, 128>(), std::integral_constant<int, OT_F16>());
-        case 12800 + OT_BF16: return f(std::integral_constant<int, 128>(), std::integral_constant<int, OT_BF16>());
-        case 6400 + OT_F32: return f(std::integral_constant<int, 64>(), std::integral_constant<int, OT_F32>());
-        case 6400 + OT_F16: return f(std::integral_constant<int, 64>(), std::integral_constant<int, OT_F16>());
-        case 6400 + OT_BF16: return f(std::integral_constant<int, 64>(), std::integral_constant<int, OT_BF16>());
-        default: return cudaErrorInvalidValue;
-    }
-}
-
 cudaError_t launch_kv8_append(const Kv8 &c, const Kv8Rows &r, const Rows &k, const Rows &v, cudaStream_t st) {
     if (r.n_seqs == 0 || r.max_rows == 0) return cudaSuccess;
     const int pages = (r.max_rows + kPage - 2) / kPage + 1;  // most pages that max_rows tokens touch

@@ -13,6 +13,7 @@
 
 #include <cuda_bf16.h>
 #include <stdint.h>
+#include <type_traits>
 
 namespace s2k {
 
@@ -135,6 +136,20 @@ __device__ __forceinline__ void store_n(T *p, bool vec, const float (&x)[N]) {
 inline bool rows_vec(const Rows &t, int n) {
     const int es = t.type == OT_F32 ? 4 : 2;
     return (uintptr_t)t.p % (size_t)(n * es) == 0 && t.row_stride % n == 0 && t.head_stride % n == 0;
+}
+
+// f(head_dim, type) as constants
+template <class F>
+cudaError_t kv8_dispatch(int hd, int type, F f) {
+    switch (hd * 100 + type) {
+        case 12800 + OT_F32: return f(std::integral_constant<int, 128>(), std::integral_constant<int, OT_F32>());
+        case 12800 + OT_F16: return f(std::integral_constant<int, 128>(), std::integral_constant<int, OT_F16>());
+        case 12800 + OT_BF16: return f(std::integral_constant<int, 128>(), std::integral_constant<int, OT_BF16>());
+        case 6400 + OT_F32: return f(std::integral_constant<int, 64>(), std::integral_constant<int, OT_F32>());
+        case 6400 + OT_F16: return f(std::integral_constant<int, 64>(), std::integral_constant<int, OT_F16>());
+        case 6400 + OT_BF16: return f(std::integral_constant<int, 64>(), std::integral_constant<int, OT_BF16>());
+        default: return cudaErrorInvalidValue;
+    }
 }
 
 struct Kv8Attn {

@@ -1,18 +1,496 @@
-// s2k_kv8_attn.cu -- attention of query rows over the 8-bit paged KV cache.
+// s2k_kv8_attn.cu -- attention of few query rows over the 8-bit paged KV cache
+// (decode steps, drafted tokens); prompts run in s2k_kv8_prompt.cu.
 //
 //   o = sum_j w_j v_j,  w = softmax over the visible keys of scale * q.k_j
 // Row i of a sequence sits at position p = past + i and sees key j iff
 //   j <= p  and  (window == 0  or  j > p - window  or  j < sinks).
 // A row that sees nothing (a sequence whose pages are all bad) is zero.
+//
+// Bound by the cache's bytes: 2 * head_dim bytes per key and kv head, read
+// once for a tile of slots, a slot being one (row, query head) pair of the kv
+// head.  At HBM's rate a page (16 keys, 4 KB at head_dim 128) leaves an SM ~700
+// issue slots, which FMAs on 4 query heads (512 per lane and page with the
+// conversions) do not fit.  So the products run on the tensor cores, and on
+// integers: the cache is int8, and a query or a weight is written in digits of
+// base 256, each a row of the left operand of mma.sync m16n8k32.
+//   S = Q K^T  rows: the digits of the slots' queries, columns: keys
+//   O = P V    rows: the digits of the slots' weights, columns: dimensions
+// 16 rows are 4 slots of 4 digits for f32 rows (30 bits: f32's accuracy) or 8
+// slots of 2 digits for f16 and bf16 (15 bits of the row's largest element and
+// of the largest weight).  Keys and values go from shared memory into the
+// products as they are, and the integer sums are exact.  The same kernel with
+// f16 products (int8 -> f16, halves of q and p) took 573 instructions per page
+// and warp, this one ~220; mma.sync does int8 at twice the rate of f16 (both 2
+// cycles per instruction and SM, measured).  tcgen05 has 128 rows: 16 of them
+// would be used, and its operands would need a pass through shared memory.
+//
+// Weights are taken relative to the largest of two pages (32 keys) with the
+// blocks' value scales in them: digits of p * v_scale / W, W the pages' largest
+// such product.  The f32 factors (W, the running maximum) multiply the sums.
+//
+// The order of dimensions within a product is free as long as both operands
+// agree.  Lane (i, c) = (lane / 4, lane % 4) takes dims 16c .. 16c+15 (and 64
+// more for head_dim 128) of a key as 16-byte words, and tokens 4c .. 4c+3 of a
+// value's dimension as one 4-byte word; the keys' columns are ordered so that
+// the weights leave S in the lane that needs them for P.
+//
+// One warp walks its own pairs of pages through its own ring of 16-byte
+// asynchronous copies with a running maximum, sum and output; no barrier inside
+// the loop.  The pages of a (tile,
+// kv head, sequence) are split over the CTAs of a cluster when there are few
+// of them, and joined through distributed shared memory: no workspace, one
+// launch, and the same order of sums every time.
 #include "s2k_common.cuh"
 #include "s2k_kv8.h"
 
-#include <type_traits>
+#include <algorithm>
+#include <atomic>
 
 namespace s2k {
 
-// One warp per (row, query head), one page of keys at a time with a running
-// maximum and sum.
+// Three CTAs of four warps per SM: a warp's step (a pair of pages) is a chain
+// of ~2000 cycles, so it takes twelve of them to keep HBM busy.  16 KB of pages
+// in flight per warp.  Twelve warps in one CTA per SM were as fast or slower
+// (a CTA's start is then hidden by no other) but for one sequence of 32768
+// tokens (22.6 against 24.7 us), which cannot fill the machine from clusters.
+constexpr int kDWarps = 4;
+constexpr int kDThreads = kDWarps * 32;
+template <int HD>
+constexpr int kDStages = HD == 128 ? 2 : 4;
+constexpr int kDMaxCluster = 16;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// D = A B + D, or + kMagicBits: int8 digits, int32 sums.  Not volatile: the
+// order among them is the compiler's.
+__device__ __forceinline__ void imma(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void imma0(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0x4b400000));
+}
+
+// The cluster's barrier in two halves: memory before the arrival is seen after the wait.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Address of `p` of this CTA's shared memory in CTA `rank` of the cluster, and stores to it.
+__device__ __forceinline__ uint32_t in_cta(const void *p, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void st_cluster(uint32_t a, float x, float y) {
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(x), "f"(y) : "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t a, float4 v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+                 : "memory");
+}
+
+// Integers below 2^22 as f32 and back by adding 1.5 * 2^23, whose low mantissa
+// bits then are the integer: conversions run at a quarter of an addition's
+// rate and took a third of the loop.
+constexpr float kMagic = 12582912.f;
+constexpr int kMagicBits = 0x4b400000;
+
+// How the 16 rows of a product are shared out.  Rows i and i + 8 are the upper
+// and lower digit of one 16-bit integer.  f32: rows i < 4 hold the high part h
+// and rows i >= 4 the low part of x = h * 2^15 + low, |h| <= 32512, |low| <=
+// 2^14, of slot i % 4.  16-bit types: x = h, of slot i.
+template <int TYPE>
+struct Digits {
+    static constexpr bool wide = TYPE == OT_F32;
+    static constexpr int slots = wide ? 4 : 8;
+    // the largest integer written: digits in [-128, 127] reach 127 * 257
+    static constexpr float unit = wide ? 32512.f * 32768.f : 32512.f;
+    static constexpr float high = 32768.f;  // wide: what an upper part's unit is worth
+    static __device__ __forceinline__ int slot(int i) { return i % slots; }
+    // the lane's part of round(x), in the low 16 bits
+    static __device__ __forceinline__ uint32_t part(float x, bool low) {
+        if (!wide) return __float_as_uint(x + kMagic);
+        const float h = fmaf(x, 1.f / high, kMagic);
+        return __float_as_uint(low ? fmaf(h - kMagic, -high, x) + kMagic : h);
+    }
+    // Four parts -> the words of their upper and lower digits.  The digits of
+    // n are the bytes of n + 0x8080, less 128 each.
+    static __device__ __forceinline__ void words(const uint32_t (&n)[4], uint32_t &a, uint32_t &b) {
+        const uint32_t s = __byte_perm(n[0] + 0x8080u, n[1] + 0x8080u, 0x4051);  // (upper, upper, lower, lower)
+        const uint32_t t = __byte_perm(n[2] + 0x8080u, n[3] + 0x8080u, 0x4051);
+        a = __byte_perm(s, t, 0x5410) ^ 0x80808080u;
+        b = __byte_perm(s, t, 0x7632) ^ 0x80808080u;
+    }
+};
+
+// (a, b) += m * (x, y) as packed f32 pairs
+__device__ __forceinline__ void fma2(float (&o)[2], float m, float x, float y) {
+    asm("{\n\t.reg .b64 d, a, b;\n\tmov.b64 d, {%0, %1};\n\tmov.b64 a, {%2, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+        "fma.rn.f32x2 d, a, b, d;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "+f"(o[0]), "+f"(o[1])
+        : "f"(m), "f"(x), "f"(y));
+}
+__device__ __forceinline__ void add2(float &x, float &y, float v) {
+    asm("{\n\t.reg .b64 d, a;\n\tmov.b64 d, {%0, %1};\n\tmov.b64 a, {%2, %2};\n\tadd.rn.f32x2 d, d, a;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(v));
+}
+
+template <int HD, int SLOTS>
+struct DecodeSmem {
+    static constexpr int kRow = HD + 8;  // eight rows' stores meet different banks
+    union {
+        alignas(128) int8_t ring[kDWarps][kDStages<HD>][2][2][kPage * HD];  // page of the pair, keys / values
+        float o[kDWarps][SLOTS][kRow];                                      // after the loop: each warp's output
+    };
+    uint32_t q[SLOTS][SLOTS == 4 ? 4 : 2][HD / 4 + 4];  // digit words of the queries, upper first
+    float qmul[SLOTS];
+    float m[kDWarps][SLOTS], l[kDWarps][SLOTS];
+    // what the cluster's CTAs send: their outputs for this CTA's share, and (maximum, sum)
+    float4 from[SLOTS * HD / 4];
+    float2 ml[kDMaxCluster][SLOTS];
+};
+
+// 16 bytes global -> shared, past L1
+__device__ __forceinline__ void cp16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// all but the last N groups of this thread have arrived
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Where byte x (16-byte aligned) of a page's keys lies in shared memory: rows
+// of 128 bytes swap their halves in odd tokens, so that the 16-byte reads of
+// two tokens' 64 bytes meet all banks.
+template <int HD>
+__device__ __forceinline__ int key_at(int x) {
+    return HD == 128 ? x ^ ((x & 128) >> 1) : x;
+}
+
+template <int HD, int TYPE>
+__global__ void __launch_bounds__(kDThreads, 3)
+    kv8_decode_kernel(Kv8 c, Kv8Rows r, Kv8Attn a, int cs_log2, float inv_group, int vec) {
+    using T = typename OType<TYPE>::T;
+    using Dg = Digits<TYPE>;
+    constexpr int SLOTS = Dg::slots, STAGES = kDStages<HD>;
+    constexpr int KV = HD / 32;  // k steps of Q K^T
+    constexpr int NU = HD / 8;   // column tiles of P V
+    constexpr unsigned kAll = 0xffffffffu;
+    extern __shared__ uint8_t raw[];
+    auto &sm = *reinterpret_cast<DecodeSmem<HD, SLOTS> *>((reinterpret_cast<uintptr_t>(raw) + 127) & ~uintptr_t(127));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, li = lane >> 2, lc = lane & 3;
+    const int cs = 1 << cs_log2, rank = blockIdx.x & (cs - 1);  // clusters lie along x
+    const int b = blockIdx.x >> cs_log2, kvh = blockIdx.y, tile = blockIdx.z;
+    const int G = a.n_heads / c.n_kv_heads;
+    int row0, n, past;
+    // the same for every CTA of the cluster: none is left waiting
+    if (!kv8_seq(r, b, row0, n, past) || tile * SLOTS >= n * G) return;
+
+    // the lane's slot; the quotient is exact below 2^20 slots
+    auto row_of = [&](int slot) { return (int)(((float)slot + 0.5f) * inv_group); };
+    const int nslots = min(SLOTS, n * G - tile * SLOTS);
+    const int ls = Dg::slot(li);
+    const int slot = tile * SLOTS + min(ls, nslots - 1);
+    const int pos = past + row_of(slot);
+    // the tile's positions, and the logical pages that one of them sees: sink
+    // pages [0, ns), then window pages [fw, ...]
+    const int pos_lo = past + row_of(tile * SLOTS), pos_hi = past + row_of(tile * SLOTS + nslots - 1);
+    const int wlo = a.window ? max(pos_lo - a.window + 1, 0) : 0;
+    const int fw = wlo / kPage;
+    const int ns = min((int)(((long long)a.sinks + kPage - 1) / kPage), fw);
+    const int total = ns + pos_hi / kPage - fw + 1;
+    // this CTA's pages, in pairs; pair k of the warp is pages 2 * (warp + k * kDWarps) and the next
+    const int pairs = (total + 1) / 2;
+    const int first = pairs * rank >> cs_log2, last = pairs * (rank + 1) >> cs_log2;
+    const int mine = last - first > warp ? (last - first - warp + kDWarps - 1) / kDWarps : 0;
+    if (cs > 1) cluster_arrive();  // this CTA runs: others may store into its shared memory
+    // lanes 2k and 2k + 1 hold pair k of the warp's current 16 pairs, and of the next 16: the physical page, or -1,
+    // and its first token, behind every position where there is no page
+    constexpr int kNone = 0x7fffff00;
+    int page, next, p0s, next_p0;
+    auto page_of = [&](int k, int &pg, int &p0) {
+        const int x = 2 * (first + warp + k * kDWarps) + (lane & 1);
+        const bool in = k < mine && x < total;
+        const int lg = x < ns ? x : x - ns + fw;
+        pg = in ? kv8_page(c, r, b, lg) : -1;
+        p0 = pg >= 0 ? lg * kPage : kNone;
+    };
+    page_of(lane >> 1, page, p0s);
+    page_of(16 + (lane >> 1), next, next_p0);
+    // pair k into its stage: every lane 16-byte pieces of both pages, one group per pair (empty behind the last)
+    auto issue = [&](int k, int pg) {
+        if (k < mine) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int p = __shfl_sync(kAll, pg, 2 * (k & 15) + e);
+                if (p < 0) continue;
+                const size_t at = c.block(p, kvh) * (kPage * HD) + lane * 16;
+                int8_t *kd = sm.ring[warp][k % STAGES][e][0], *vd = sm.ring[warp][k % STAGES][e][1];
+#pragma unroll
+                for (int x = 0; x < HD / 32; ++x) {
+                    cp16(kd + key_at<HD>(lane * 16 + x * 512), c.k + at + x * 512);
+                    cp16(vd + lane * 16 + x * 512, c.v + at + x * 512);
+                }
+            }
+        }
+        cp_commit();
+    };
+#pragma unroll
+    for (int k = 0; k < STAGES - 1; ++k) issue(k, page);
+
+    // queries in digits, a warp a slot at a time: lane l dims [l * E, l * E + E)
+    {
+        constexpr int E = HD / 32;
+        for (int sl = warp; sl < SLOTS; sl += kDWarps) {
+            const int st = tile * SLOTS + min(sl, nslots - 1), row = row_of(st);
+            float x[E];
+            load_n<E>(reinterpret_cast<const T *>(a.q.p) + (long long)(row0 + row) * a.q.row_stride +
+                          (long long)(kvh * G + st - row * G) * a.q.head_stride + lane * E,
+                      vec, x);
+            unsigned top = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+            top = __reduce_max_sync(kAll, top);
+            // the row's largest element becomes `unit`; rows below 2^-90 as if they had one of that size
+            const float amax = fmaxf(__uint_as_float(top), 8.0779356694631609e-28f);
+            const float up = __fdividef(Dg::unit, amax);
+            if (lane == 0) sm.qmul[sl] = top >= 0x7f800000u ? NAN : a.scale * 1.44269504f * __fdiv_rn(1.f, up);
+            uint32_t v[4] = {}, w[4];
+#pragma unroll
+            for (int h = 0; h < (Dg::wide ? 2 : 1); ++h) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = Dg::part(x[e] * up, h);
+                Dg::words(v, w[2 * h], w[2 * h + 1]);
+            }
+#pragma unroll
+            for (int d = 0; d < (Dg::wide ? 4 : 2); ++d) {
+                if (E == 4) sm.q[sl][d][lane] = w[d];
+                else reinterpret_cast<uint16_t *>(sm.q[sl][d])[lane] = (uint16_t)w[d];
+            }
+        }
+    }
+    __syncthreads();
+    uint32_t q[KV][4];
+    const float smul = sm.qmul[ls];  // takes the scores to base-2 logarithms
+#pragma unroll
+    for (int j = 0; j < KV / 2; ++j)
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(&sm.q[ls][(Dg::wide && li >= 4 ? 2 : 0) + d][16 * j + 4 * lc]);
+            q[2 * j][d] = w.x;
+            q[2 * j][2 + d] = w.y;
+            q[2 * j + 1][d] = w.z;
+            q[2 * j + 1][2 + d] = w.w;
+        }
+    float m = -INFINITY, l = 0.f;  // l: this lane's tokens only
+    float o[NU][2];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) o[u][0] = o[u][1] = 0.f;
+    float ks = 0.f, vs = 0.f;
+    for (int k = 0; k < mine; ++k) {
+        if (k % 16 == 0) {
+            if (k) {
+                page = next;
+                p0s = next_p0;
+                page_of(k + 16 + (lane >> 1), next, next_p0);
+            }
+            ks = vs = 0.f;
+            if (page >= 0) {  // wanted only once the page itself has come
+                ks = c.k_scale[c.block(page, kvh)];
+                vs = c.v_scale[c.block(page, kvh)];
+            }
+        }
+        const int s = k % STAGES, from = 2 * (k & 15);
+        __syncwarp();  // every lane has read the stage that comes next
+        const int ahead = k + STAGES - 1;
+        issue(ahead, (ahead >> 4) == (k >> 4) ? page : next);
+        cp_wait<STAGES - 1>();
+        __syncwarp();  // the pair has arrived for every lane
+        // scores of the pair: x[4 e + t] is token 4 lc + t of page e
+        float x[8], pm[2], f[2];
+        int p0[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int8_t *kp = sm.ring[warp][s][e][0];
+            const float pks = __shfl_sync(kAll, ks, from + e) * smul;
+            f[e] = __shfl_sync(kAll, vs, from + e);
+            p0[e] = __shfl_sync(kAll, p0s, from + e);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                int acc[4];
+                const int tok = 4 * (li >> 1) + 2 * t + (li & 1);
+#pragma unroll
+                for (int j = 0; j < KV / 2; ++j) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(kp + key_at<HD>(tok * HD + 64 * j + 16 * lc));
+                    if (j == 0) imma0(acc, q[0], w.x, w.y);
+                    else imma(acc, q[2 * j], w.x, w.y);
+                    imma(acc, q[2 * j + 1], w.z, w.w);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float y = fmaf(__int_as_float(acc[h]) - kMagic, 256.f, __int_as_float(acc[2 + h]) - kMagic);
+                    if (Dg::wide) {
+                        const float other = __shfl_xor_sync(kAll, y, 16);
+                        y = li < 4 ? fmaf(y, Dg::high, other) : fmaf(other, Dg::high, y);
+                    }
+                    x[4 * e + 2 * t + h] = y * pks;
+                }
+            }
+        }
+        // a page at the edge of what the slots see, or none
+        const int p_lo = min(p0[0], p0[1]), p_hi = max(p0[0], p0[1]);
+        if (p_hi + kPage - 1 > pos_lo || (a.window && p_lo <= pos_hi - a.window && p_hi + kPage > a.sinks)) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (!(p0[e] <= pos && (!a.window || p0[e] + kPage - 1 > pos - a.window || p0[e] < a.sinks)))
+                    f[e] = 0.f;  // a hidden block's scale may be NaN
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const int j = p0[e] + 4 * lc + t;
+                    if (j > pos || (a.window && j <= pos - a.window && j >= a.sinks)) x[4 * e + t] = -INFINITY;
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float t = fmaxf(fmaxf(x[4 * e], x[4 * e + 1]), fmaxf(x[4 * e + 2], x[4 * e + 3]));
+            t = fmaxf(t, __shfl_xor_sync(kAll, t, 1));
+            pm[e] = fmaxf(t, __shfl_xor_sync(kAll, t, 2));
+        }
+        const float both = fmaxf(pm[0], pm[1]);
+        const float ref = both == -INFINITY ? 0.f : both;
+        const float m2 = fmaxf(m, both);
+        if (__any_sync(kAll, m2 > m)) {
+            const float alpha = m == m2 ? 1.f : ex2(m - m2);  // 0 for the slot's first pair
+            l *= alpha;
+#pragma unroll
+            for (int u = 0; u < NU; ++u) o[u][0] *= alpha, o[u][1] *= alpha;
+            m = m2;
+        }
+        const float f0 = both == -INFINITY ? 0.f : ex2(ref - m2);
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = ex2(x[e] - ref);
+        l += f0 * (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
+        // weights times value scales, relative to the pair's largest; a NaN scale has to reach the sum by `down`:
+        // integers do not carry it
+        const float W = fmaxf(fmaxf(ex2(pm[0] - ref) * f[0], ex2(pm[1] - ref) * f[1]), 7.8886090522101181e-31f);
+        const float up = __fdividef(Dg::unit, W);
+        const float down = f0 * (W * (1.f / Dg::unit)) + 0.f * (f[0] + f[1]);
+        uint32_t pa[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            uint32_t v[4];
+            const float g = f[e] * up;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) v[t] = Dg::part(p[4 * e + t] * g, li >= 4);
+            Dg::words(v, pa[2 * e], pa[2 * e + 1]);
+        }
+        const float mul = Dg::wide && li < 4 ? down * Dg::high : down;
+        const int8_t *v0 = sm.ring[warp][s][0][1] + lane * 4, *v1 = sm.ring[warp][s][1][1] + lane * 4;
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            int d[4];
+            imma0(d, pa, *reinterpret_cast<const uint32_t *>(v0 + u * 128), *reinterpret_cast<const uint32_t *>(v1 + u * 128));
+            float y[4] = {__int_as_float(d[0]), __int_as_float(d[1]), __int_as_float(d[2]), __int_as_float(d[3])};
+            add2(y[0], y[1], -kMagic);
+            add2(y[2], y[3], -kMagic);
+            fma2(o[u], mul * 256.f, y[0], y[1]);
+            fma2(o[u], mul, y[2], y[3]);
+        }
+    }
+    l += __shfl_xor_sync(kAll, l, 1);
+    l += __shfl_xor_sync(kAll, l, 2);
+    if (Dg::wide) {  // upper and lower digits
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            o[u][0] += __shfl_xor_sync(kAll, o[u][0], 16);
+            o[u][1] += __shfl_xor_sync(kAll, o[u][1], 16);
+        }
+    }
+
+    // join the warps, in order: outputs relative to the CTA's maximum
+    if (li < SLOTS && lc == 0) sm.m[warp][ls] = m;
+    cp_wait<0>();
+    __syncthreads();  // the maxima are there, and the ring is read
+    float top = sm.m[0][ls];
+#pragma unroll
+    for (int w = 1; w < kDWarps; ++w) top = fmaxf(top, sm.m[w][ls]);
+    const float g = m == -INFINITY ? 0.f : ex2(m - top);
+    if (li < SLOTS) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+            *reinterpret_cast<float2 *>(&sm.o[warp][ls][8 * u + 2 * lc]) = make_float2(g * o[u][0], g * o[u][1]);
+        if (lc == 0) sm.l[warp][ls] = g * l;  // NaN scores leave m at -inf and l NaN: 0 * NaN is NaN
+    }
+    __syncthreads();
+    constexpr int kItems = SLOTS * HD / 4;  // of 4 dims; with a cluster each CTA joins a share of them
+    const int share = kItems >> cs_log2;
+    auto put = [&](int item, float sum, float4 v) {
+        const int st = tile * SLOTS + item / (HD / 4);
+        if (item / (HD / 4) >= nslots) return;
+        const int row = row_of(st);
+        const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+        const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+        store_n<4>(reinterpret_cast<T *>(a.out.p) + (long long)(row0 + row) * a.out.row_stride +
+                       (long long)(kvh * G + st - row * G) * a.out.head_stride + item % (HD / 4) * 4,
+                   vec, y);
+    };
+    if (cs > 1) cluster_wait();
+    for (int item = tid; item < kItems; item += kDThreads) {
+        const int sl = item / (HD / 4), d = item % (HD / 4) * 4;
+        float4 v = *reinterpret_cast<const float4 *>(&sm.o[0][sl][d]);
+        float sum = sm.l[0][sl];
+#pragma unroll
+        for (int w = 1; w < kDWarps; ++w) {
+            const float4 t = *reinterpret_cast<const float4 *>(&sm.o[w][sl][d]);
+            v = make_float4(v.x + t.x, v.y + t.y, v.z + t.z, v.w + t.w);
+            sum += sm.l[w][sl];
+        }
+        if (cs == 1) put(item, sum, v);
+        else st_cluster(in_cta(&sm.from[rank * share + item % share], item / share), v);
+    }
+    if (cs == 1) return;
+    for (int x = tid; x < SLOTS * cs; x += kDThreads) {
+        const int sl = x % SLOTS;
+        float mm = sm.m[0][sl], sum = sm.l[0][sl];
+#pragma unroll
+        for (int w = 1; w < kDWarps; ++w) mm = fmaxf(mm, sm.m[w][sl]), sum += sm.l[w][sl];
+        st_cluster(in_cta(&sm.ml[rank][sl], x / SLOTS), mm, sum);
+    }
+    cluster_arrive();
+    cluster_wait();  // from here no CTA reaches into another's shared memory
+    for (int x = tid; x < share; x += kDThreads) {
+        const int item = rank * share + x, sl = item / (HD / 4);
+        float mm = -INFINITY, sum = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int k = 0; k < cs; ++k) mm = fmaxf(mm, sm.ml[k][sl].x);
+#pragma unroll 4
+        for (int k = 0; k < cs; ++k) {
+            const float2 ml = sm.ml[k][sl];
+            const float4 t = sm.from[k * share + x];
+            const float gk = ml.x == -INFINITY ? 0.f : ex2(ml.x - mm);
+            sum += gk * ml.y;
+            v = make_float4(v.x + gk * t.x, v.y + gk * t.y, v.z + gk * t.z, v.w + gk * t.w);
+        }
+        put(item, sum, v);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// One warp per (row, query head), one page of keys at a time: prompts, until
+// they have a kernel of their own.
 template <int HD, int TYPE>
 __global__ void __launch_bounds__(128) kv8_attn_simple_kernel(Kv8 c, Kv8Rows r, Kv8Attn a) {
     using T = typename OType<TYPE>::T;
@@ -80,20 +558,89 @@ __global__ void __launch_bounds__(128) kv8_attn_simple_kernel(Kv8 c, Kv8Rows r, 
                false, o);
 }
 
-cudaError_t launch_kv8_attend(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, cudaStream_t st) {
-    if (r.n_seqs == 0 || r.max_rows == 0) return cudaSuccess;
+static cudaError_t launch_simple(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, cudaStream_t st) {
     const dim3 grid(r.max_rows, (a.n_heads + 3) / 4, r.n_seqs);
     count_launch();
-    switch (c.head_dim * 100 + a.q.type) {
-        case 12800 + OT_F32: kv8_attn_simple_kernel<128, OT_F32><<<grid, 128, 0, st>>>(c, r, a); break;
-        case 12800 + OT_F16: kv8_attn_simple_kernel<128, OT_F16><<<grid, 128, 0, st>>>(c, r, a); break;
-        case 12800 + OT_BF16: kv8_attn_simple_kernel<128, OT_BF16><<<grid, 128, 0, st>>>(c, r, a); break;
-        case 6400 + OT_F32: kv8_attn_simple_kernel<64, OT_F32><<<grid, 128, 0, st>>>(c, r, a); break;
-        case 6400 + OT_F16: kv8_attn_simple_kernel<64, OT_F16><<<grid, 128, 0, st>>>(c, r, a); break;
-        case 6400 + OT_BF16: kv8_attn_simple_kernel<64, OT_BF16><<<grid, 128, 0, st>>>(c, r, a); break;
-        default: return cudaErrorInvalidValue;
+    return kv8_dispatch(c.head_dim, a.q.type, [&](auto hd, auto type) {
+        kv8_attn_simple_kernel<hd, type><<<grid, 128, 0, st>>>(c, r, a);
+        return cudaGetLastError();
+    });
+}
+
+// What a device allows, looked up once.
+struct DecodeDevice {
+    std::atomic<int> ready{0};
+    int sms = 148;
+};
+static DecodeDevice g_decode[64];
+
+template <int HD, int TYPE>
+static constexpr int decode_smem() {
+    return (int)sizeof(DecodeSmem<HD, Digits<TYPE>::slots>) + 128;
+}
+
+template <int HD, int TYPE>
+static cudaError_t decode_setup() {
+    const auto f = kv8_decode_kernel<HD, TYPE>;
+    cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, decode_smem<HD, TYPE>());
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+}
+
+template <int HD, int TYPE>
+static cudaError_t decode_launch(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, int cs_log2, int tiles,
+                                 cudaStream_t st) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1u << cs_log2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)r.n_seqs << cs_log2, c.n_kv_heads, tiles);
+    cfg.blockDim = dim3(kDThreads);
+    cfg.dynamicSmemBytes = decode_smem<HD, TYPE>();
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = cs_log2 > 0 ? 1 : 0;
+    const float inv_group = 1.0f / (float)(a.n_heads / c.n_kv_heads);
+    const int vec = rows_vec(a.q, 4) && rows_vec(a.out, 4);
+    return cudaLaunchKernelEx(&cfg, kv8_decode_kernel<HD, TYPE>, c, r, a, cs_log2, inv_group, vec);
+}
+
+cudaError_t launch_kv8_attend(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, cudaStream_t st) {
+    if (r.n_seqs == 0 || r.max_rows == 0) return cudaSuccess;
+    const int G = a.n_heads / c.n_kv_heads;
+    if ((long long)r.max_rows * G > 64) return launch_simple(c, r, a, st);
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64) return cudaErrorInvalidDevice;
+    DecodeDevice &d = g_decode[dev];
+    if (!d.ready.load(std::memory_order_acquire)) {
+        // idempotent: threads that meet here set the same values
+        int sms = 0;
+        if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev))) return e;
+        for (int hd : {64, 128})
+            for (int type : {OT_F32, OT_F16, OT_BF16})
+                if ((e = kv8_dispatch(hd, type, [&](auto h, auto t) { return decode_setup<h, t>(); }))) return e;
+        d.sms = sms;
+        d.ready.store(1, std::memory_order_release);
     }
-    return cudaGetLastError();
+    const int slots = a.q.type == OT_F32 ? Digits<OT_F32>::slots : Digits<OT_F16>::slots;
+    const int tiles = (r.max_rows * G + slots - 1) / slots;
+    const long long units = (long long)tiles * c.n_kv_heads * r.n_seqs;
+    // pages of one unit at most
+    long long pages = r.table_ld;
+    if (a.window) pages = std::min(pages, ((long long)a.window + r.max_rows + a.sinks) / kPage + 3);
+    // CTAs per unit.  A CTA's start and its join cost about as much as 40 pages, so pieces of 48 to 96 pages are
+    // best where the machine is full (64 sequences of up to 2523 tokens: 45.6 us whole, 42.9 halved, 51 in
+    // quarters; 8 of up to 6095: 28.7 halved, 20.5 quartered, 23.3 in eighths); with SMs left over, down to one
+    // pair of pages per warp (one sequence of 512 tokens: 6.7 us in the kernel whole, 5.1 in pieces).
+    int cs = 0;
+    while (cs < 4 && (pages > 96LL << cs || (units << (cs + 1) <= d.sms && pages > 8LL << cs))) ++cs;
+    if ((long long)r.n_seqs << cs > 0x7fffffffLL) return cudaErrorInvalidValue;
+    count_launch();
+    return kv8_dispatch(c.head_dim, a.q.type, [&](auto hd, auto type) {
+        return decode_launch<hd, type>(c, r, a, cs, tiles, st);
+    });
 }
 
 }  // namespace s2k

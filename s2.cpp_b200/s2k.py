@@ -873,40 +873,45 @@ class CodecStream:
 
 
 # --- operators on device memory: torch CUDA tensors in and out, on the current stream ---
+#
+# A decode step's operators take a few microseconds on the device, so the
+# checks here stay cheap: torch's dtype objects are compared by identity (the
+# module is looked up at the first call, the binding does not need it before).
 
-_OP_TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 30}  # S2K_TYPE_F32 / F16 / BF16
-_op_type_of = {}  # torch dtype -> S2K_TYPE_*
+_torch = None
+_OP_TYPES = {}  # torch dtype -> S2K_TYPE_F32 / F16 / BF16
+_raw_stream = None
+
+
+def _torch_module():
+    global _torch, _raw_stream
+    if _torch is None:
+        import torch
+        _OP_TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 30})
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda device: torch.cuda.current_stream(device).cuda_stream)
+        _torch = torch
+    return _torch
 
 
 def _op_type(what: str, t) -> int:
-    code = _op_type_of.get(t.dtype)
+    code = _OP_TYPES.get(t.dtype)
     if code is None:
-        code = _OP_TYPES.get(str(t.dtype))
-        if code is None:
-            raise S2KError(-7, f"{what} has type {t.dtype} (float32, float16 or bfloat16)")
-        _op_type_of[t.dtype] = code
+        raise S2KError(-7, f"{what} has type {t.dtype} (float32, float16 or bfloat16)")
     return code
 
 
 def _op_stream(device: int, stream) -> int:
-    if stream is None:
-        import torch
-        return torch.cuda.current_stream(device).cuda_stream
-    return int(getattr(stream, "cuda_stream", stream))
-
-
-def _on_device(what: str, t, device: int) -> int:
-    """Data pointer of a CUDA tensor of `device`."""
-    if t.get_device() != device:
-        raise S2KError(-1, f"{what} is not on CUDA device {device}")
-    return t.data_ptr()
+    return _raw_stream(device) if stream is None else int(getattr(stream, "cuda_stream", stream))
 
 
 def _ints(what: str, t, shape, device: int) -> int:
-    """Data pointer of a contiguous int32 tensor."""
-    if str(t.dtype) != "torch.int32" or tuple(t.shape) != shape or not t.is_contiguous():
+    """Data pointer of a contiguous int32 tensor of `device`."""
+    if t.dtype is not _torch.int32 or t.shape != shape or not t.is_contiguous():
         raise S2KError(-1, f"{what} must be a contiguous int32 tensor of shape {list(shape)}")
-    return _on_device(what, t, device)
+    if t.get_device() != device:
+        raise S2KError(-1, f"{what} is not on CUDA device {device}")
+    return t.data_ptr()
 
 
 class KV8Cache:
@@ -930,20 +935,22 @@ class KV8Cache:
     PAGE = 16
 
     def __init__(self, k, v, k_scale, v_scale):
+        T = _torch or _torch_module()
         if k.dim() != 5 or k.shape[3] != 16:
             raise S2KError(-1, "k must be int8 [pages][layers][kv_heads][16][head_dim]")
         P, L, H, _, D = k.shape
-        self.device = k.get_device()
-        for what, t, dtype, shape in (("k", k, "torch.int8", (P, L, H, 16, D)), ("v", v, "torch.int8", (P, L, H, D, 16)),
-                                      ("k_scale", k_scale, "torch.float32", (P, L, H)),
-                                      ("v_scale", v_scale, "torch.float32", (P, L, H))):
-            if str(t.dtype) != dtype or tuple(t.shape) != shape or not t.is_contiguous():
-                raise S2KError(-1, f"{what} must be a contiguous {dtype[6:]} tensor of shape {list(shape)}")
-            if self.device < 0 or t.get_device() != self.device:
+        self.device = device = k.get_device()
+        for what, t, dtype, shape in (("k", k, T.int8, (P, L, H, 16, D)), ("v", v, T.int8, (P, L, H, D, 16)),
+                                      ("k_scale", k_scale, T.float32, (P, L, H)),
+                                      ("v_scale", v_scale, T.float32, (P, L, H))):
+            if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+                raise S2KError(-1, f"{what} must be a contiguous {dtype} tensor of shape {list(shape)}")
+            if device < 0 or t.get_device() != device:
                 raise S2KError(-1, f"{what} is not on the CUDA device of the cache")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_pages, self.n_layers, self.n_kv_heads, self.head_dim = P, L, H, D
-        self._c = _KV8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.device, P, L, H, D)
+        self._c = c = _KV8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), device, P, L, H, D)
+        self._ref = ctypes.byref(c)
 
     @classmethod
     def empty(cls, n_pages: int, n_layers: int, n_kv_heads: int, head_dim: int, device: int = 0) -> "KV8Cache":
@@ -969,10 +976,15 @@ class KV8Cache:
                         None if err is None else _ints("err", err, (1,), dev))
 
     def _heads(self, what: str, t, n_heads) -> _Heads:
-        s = t.stride() if t.dim() != 3 or t.shape[0] else (t.shape[1] * t.shape[2], t.shape[2], 1)  # no rows: any
-        if len(s) != 3 or t.shape[2] != self.head_dim or (n_heads is not None and t.shape[1] != n_heads) or s[2] != 1:
+        shape, s = t.shape, t.stride()
+        if len(s) != 3 or shape[2] != self.head_dim or (n_heads is not None and shape[1] != n_heads) or \
+                (s[2] != 1 and shape[0]):
             raise S2KError(-1, f"{what} must be [rows][heads][{self.head_dim}] with a dense last dimension")
-        return _Heads(_on_device(what, t, self.device), s[0], s[1], _op_type(what, t))
+        if t.get_device() != self.device:
+            raise S2KError(-1, f"{what} is not on CUDA device {self.device}")
+        if not shape[0]:
+            s = (shape[1] * shape[2], shape[2], 1)  # no rows: whatever their strides
+        return _Heads(t.data_ptr(), s[0], s[1], _op_type(what, t))
 
     def append(self, layer: int, k, v, past, block_table, row_start=None, max_rows: Optional[int] = None, err=None,
                stream=None) -> None:
@@ -981,7 +993,7 @@ class KV8Cache:
             raise S2KError(-1, "k and v have different shapes")
         r = self._rows(k.shape[0], past, block_table, row_start, max_rows, err)
         kh, vh = self._heads("k", k, self.n_kv_heads), self._heads("v", v, self.n_kv_heads)
-        _check(lib().s2k_kv8_append(ctypes.byref(self._c), layer, ctypes.byref(r), ctypes.byref(kh), ctypes.byref(vh),
+        _check(lib().s2k_kv8_append(self._ref, layer, ctypes.byref(r), ctypes.byref(kh), ctypes.byref(vh),
                                     _op_stream(self.device, stream)))
 
     def read(self, layer: int, n_rows: int, past, block_table, row_start=None, max_rows: Optional[int] = None,
@@ -996,7 +1008,7 @@ class KV8Cache:
             raise S2KError(-1, f"out must hold {n_rows} rows")
         r = self._rows(n_rows, past, block_table, row_start, max_rows, err)
         kh, vh = self._heads("k", out[0], self.n_kv_heads), self._heads("v", out[1], self.n_kv_heads)
-        _check(lib().s2k_kv8_read(ctypes.byref(self._c), layer, ctypes.byref(r), ctypes.byref(kh), ctypes.byref(vh),
+        _check(lib().s2k_kv8_read(self._ref, layer, ctypes.byref(r), ctypes.byref(kh), ctypes.byref(vh),
                                   _op_stream(self.device, stream)))
         return out[0], out[1]
 
@@ -1013,7 +1025,7 @@ class KV8Cache:
         qh, oh = self._heads("q", q, None), self._heads("out", out, None)
         if scale is None:
             scale = self.head_dim ** -0.5
-        _check(lib().s2k_kv8_attend(ctypes.byref(self._c), layer, ctypes.byref(r), ctypes.byref(qh), ctypes.byref(oh),
+        _check(lib().s2k_kv8_attend(self._ref, layer, ctypes.byref(r), ctypes.byref(qh), ctypes.byref(oh),
                                     q.shape[1], scale, window, sinks, _op_stream(self.device, stream)))
         return out
 
@@ -1022,22 +1034,22 @@ def logprobs(logits, targets=None, n_top: int = 0, stream=None):
     """(logprob [rows], entropy [rows], top_ids [rows][n_top], top_logprobs [rows][n_top]) of logits [rows][n]
     (s2k_logprobs): the log probability of each row's target (int32 CUDA tensor [rows]; None without targets), the
     entropy in nats, and the n_top (<= 32) most likely tokens, ties to the lowest index (both None for n_top 0)."""
+    T = _torch or _torch_module()
     if logits.dim() != 2 or logits.shape[1] == 0 or (logits.shape[0] and logits.stride(1) != 1):
         raise S2KError(-1, "logits must be [rows][n] with a dense last dimension")
-    import torch
     rows, n = logits.shape
     dev, code = logits.get_device(), _op_type("logits", logits)
-    x = _on_device("logits", logits, dev) if dev >= 0 else None
-    if x is None:
+    if dev < 0:
         raise S2KError(-1, "logits is not on a CUDA device")
     tgt = None if targets is None else _ints("targets", targets, (rows,), dev)
-    res = logits.new_empty((2, rows), dtype=torch.float32)
+    logprob = None if targets is None else logits.new_empty(rows, dtype=T.float32)
+    entropy = logits.new_empty(rows, dtype=T.float32)
     ids = top = None
     if n_top > 0:
-        ids = logits.new_empty((rows, n_top), dtype=torch.int32)
-        top = logits.new_empty((rows, n_top), dtype=torch.float32)
-    _check(lib().s2k_logprobs(dev, x, code, rows, n, max(logits.stride(0), 0), tgt, n_top,
-                              None if tgt is None else res.data_ptr(), res.data_ptr() + 4 * rows,
+        ids = logits.new_empty((rows, n_top), dtype=T.int32)
+        top = logits.new_empty((rows, n_top), dtype=T.float32)
+    _check(lib().s2k_logprobs(dev, logits.data_ptr(), code, rows, n, max(logits.stride(0), 0), tgt, n_top,
+                              None if logprob is None else logprob.data_ptr(), entropy.data_ptr(),
                               None if ids is None else ids.data_ptr(), None if top is None else top.data_ptr(),
                               _op_stream(dev, stream)))
-    return (None if tgt is None else res[0]), res[1], ids, top
+    return logprob, entropy, ids, top

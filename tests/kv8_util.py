@@ -65,12 +65,15 @@ def seen(pos, n, window, sinks):
     return (j <= pos) & ((window == 0) | (j > pos - window) | (j < sinks))
 
 
-def attend(k, v, q, past, scale, window=0, sinks=0):
-    """One sequence: k, v [n][Hkv][dim], q [T][H][dim] at positions past..; returns (out, bound) [T][H][dim], bound
-    the summed |weight * value| and each row's largest scale * sum |q k| (the scores' size)."""
+def attend(k, v, q, past, scale, window=0, sinks=0, vtop=None):
+    """One sequence: k, v [n][Hkv][dim], q [T][H][dim] at positions past...  Returns out [T][H][dim]; the summed
+    |weight * value| [T][H][dim]; each row's largest scale * sum |q k| (the scores' size); its largest scale * max|q| *
+    sum |k|; and the sum over pages of 2 * 32 * (the page's largest weight * vtop), vtop [n][Hkv] what a position's
+    block can hold at most (a pair's largest is at most the sum of its two pages', twice for either pairing)."""
     T, H, D = q.shape
     G = H // k.shape[1]
-    out, mag, size = np.zeros((T, H, D)), np.zeros((T, H, D)), np.zeros((T, H))
+    out, mag = np.zeros((T, H, D)), np.zeros((T, H, D))
+    size, reach, grain = np.zeros((T, H)), np.zeros((T, H)), np.zeros((T, H))
     for i in range(T):
         m = seen(past + i, k.shape[0], window, sinks)
         if not m.any():
@@ -79,8 +82,13 @@ def attend(k, v, q, past, scale, window=0, sinks=0):
             kk, vv = k[m, h // G], v[m, h // G]
             s = kk @ q[i, h] * scale
             size[i, h] = (np.abs(kk) @ np.abs(q[i, h])).max() * abs(scale)
+            reach[i, h] = np.abs(kk).sum(1).max() * np.abs(q[i, h]).max() * abs(scale)
             w = np.exp(s - s.max())
             w /= w.sum()
             out[i, h] = w @ vv
             mag[i, h] = w @ np.abs(vv)
-    return out, mag, size
+            if vtop is not None:
+                x = np.zeros((k.shape[0] + PAGE - 1) // PAGE * PAGE)
+                x[: k.shape[0]][m] = w * vtop[m, h // G]
+                grain[i, h] = 64 * x.reshape(-1, PAGE).max(1).sum()
+    return out, mag, size, reach, grain

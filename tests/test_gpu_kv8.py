@@ -3,11 +3,18 @@
 
 Tolerances.  append / read: the stored integers are defined exactly (the
 quotient correctly rounded), so integers and scales must be equal.  attend:
-with e the score's size (scale * sum |q k|), a score summed in f32 is off by
-at most 2^-20 e, which moves each weight by twice that, relative; the weights'
-exponentials and sums add 2^-18.  Both scale the summed |w v|.  16-bit types
-add the rounding of the weights to f16 (2^-11, numerator and its sum) and the
-result's own half step (f16 2^-11, bf16 2^-8)."""
+the score's size is e = scale * sum |q k|.  f32 rows: a score is off by at most
+2^-20 e (sums in f32 or exacter), which moves each weight by twice that,
+relative; the weights' exponentials and sums add 2^-18; both scale the summed
+|w v|.  16-bit rows: a query's elements are held to 2^-16 of its largest, which
+moves a score by up to 2^-16 * scale * max|q| * sum |k|, and a weight by twice
+that; the weights' rounding to f16 in the prompt kernel adds 2^-11 twice
+(numerator and sum), the result its own half step (f16 2^-11, bf16 2^-8).
+Weights are held in fixed point relative to the largest of their pair of pages
+(32 keys): to 2^-16 of it for 16-bit rows, 2^-30 for f32 ones, whatever their
+own size; for the 32 keys together 32 * that * (the pair's largest weight times
+value scale) * 127, which `grain` sums over all pairs (of either parity).
+"""
 from __future__ import annotations
 
 import numpy as np
@@ -21,6 +28,8 @@ pytestmark = pytest.mark.gpu
 
 DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 HALF_STEP = {"f32": 2.0**-24, "f16": 2.0**-11, "bf16": 2.0**-8}
+GRAIN = {"f32": 2.0**-30, "f16": 2.0**-16, "bf16": 2.0**-16}
+QUERY = {"f32": 0.0, "f16": 2.0**-16, "bf16": 2.0**-16}
 EXTRA = {"f32": 2.0**-18, "f16": 2.0**-18 + 2 * 2.0**-11, "bf16": 2.0**-18 + 2 * 2.0**-11}
 
 
@@ -71,8 +80,10 @@ class Call:
             k = ku.values(self.kq, self.ks, self.layer, self.table[b], p + t, False)
             v = ku.values(self.vq, self.vs, self.layer, self.table[b], p + t, True)
             sl = slice(self.start[b], self.start[b + 1])
-            want, mag, size = ku.attend(k, v, qn[sl], p, scale, window, sinks)
-            tol = mag * (2 * 2.0**-20 * size[..., None] + EXTRA[self.typ]) + np.abs(want) * HALF_STEP[self.typ] * 1.01 + 1e-30
+            vtop = np.repeat(self.vs[self.table[b, : (p + t + 15) // 16], self.layer].astype(np.float64), 16, 0)[: p + t] * 127
+            want, mag, size, reach, grain = ku.attend(k, v, qn[sl], p, scale, window, sinks, vtop)
+            score = 2.0**-20 * size + QUERY[self.typ] * reach
+            tol = GRAIN[self.typ] * grain[..., None] + mag * (2 * score[..., None] + EXTRA[self.typ]) + np.abs(want) * HALF_STEP[self.typ] * 1.01 + 1e-30
             d = np.abs(on[sl] - want)
             assert np.all(d <= tol), f"sequence {b}: {np.nanmax(d / tol)} times the tolerance"
 
@@ -284,7 +295,7 @@ def test_far_pages_pass_32_bit_offsets():
     q = torch.randn(40, 4, D, device="cuda")
     out = cache.attend(0, q, i32([0]), table)
     one = cache.attend(0, q[39:], i32([39]), table)
-    want, mag, size = ku.attend(kb.double().cpu().numpy(), vb.double().cpu().numpy(), q.double().cpu().numpy(), 0, D ** -0.5)
+    want, mag, size, _, _ = ku.attend(kb.double().cpu().numpy(), vb.double().cpu().numpy(), q.double().cpu().numpy(), 0, D ** -0.5)
     tol = mag * (2 * 2.0**-20 * size[..., None] + EXTRA["f32"]) + np.abs(want) * 2.0**-24 * 2
     assert np.all(np.abs(out.double().cpu().numpy() - want) <= tol)
     assert np.all(np.abs(one[0].double().cpu().numpy() - want[39]) <= tol[39])
