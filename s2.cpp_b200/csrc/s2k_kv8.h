@@ -9,6 +9,7 @@
 // operand the tensor cores take.
 #pragma once
 
+#include "s2k_common.cuh"
 #include "s2k_kernels.h"
 
 #include <cuda_bf16.h>
@@ -98,6 +99,47 @@ __device__ __forceinline__ __half from_f<__half>(float x) {
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) {
     return __float2bfloat16_rn(x);
+}
+
+// 2^x; subnormal results are zero
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Most CTAs of a cluster that the operators use (more than 8 is opt-in).
+constexpr int kMaxCluster = 16;
+
+// The cluster's barrier in two halves: memory before the arrival is seen after the wait.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Address of `p` of this CTA's shared memory in CTA `rank` of the cluster, and stores to it.
+__device__ __forceinline__ uint32_t in_cta(const void *p, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void st_cluster(uint32_t a, float x, float y) {
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(x), "f"(y) : "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t a, float4 v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+                 : "memory");
+}
+
+// (a, b) += m * (x, y) as packed f32 pairs
+__device__ __forceinline__ void fma2(float (&o)[2], float m, float x, float y) {
+    asm("{\n\t.reg .b64 d, a, b;\n\tmov.b64 d, {%0, %1};\n\tmov.b64 a, {%2, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+        "fma.rn.f32x2 d, a, b, d;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "+f"(o[0]), "+f"(o[1])
+        : "f"(m), "f"(x), "f"(y));
+}
+__device__ __forceinline__ void add2(float &x, float &y, float v) {
+    asm("{\n\t.reg .b64 d, a;\n\tmov.b64 d, {%0, %1};\n\tmov.b64 a, {%2, %2};\n\tadd.rn.f32x2 d, d, a;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(v));
 }
 
 template <class T, int N>

@@ -57,14 +57,6 @@ constexpr int kDWarps = 4;
 constexpr int kDThreads = kDWarps * 32;
 template <int HD>
 constexpr int kDStages = HD == 128 ? 2 : 4;
-constexpr int kDMaxCluster = 16;
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // D = A B + D, or + kMagicBits: int8 digits, int32 sums.  Not volatile: the
 // order among them is the compiler's.
 __device__ __forceinline__ void imma(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -76,23 +68,6 @@ __device__ __forceinline__ void imma0(int (&d)[4], const uint32_t (&a)[4], uint3
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0x4b400000));
-}
-
-// The cluster's barrier in two halves: memory before the arrival is seen after the wait.
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// Address of `p` of this CTA's shared memory in CTA `rank` of the cluster, and stores to it.
-__device__ __forceinline__ uint32_t in_cta(const void *p, uint32_t rank) {
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-    return a;
-}
-__device__ __forceinline__ void st_cluster(uint32_t a, float x, float y) {
-    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(x), "f"(y) : "memory");
-}
-__device__ __forceinline__ void st_cluster(uint32_t a, float4 v) {
-    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
-                 : "memory");
 }
 
 // Integers below 2^22 as f32 and back by adding 1.5 * 2^23, whose low mantissa
@@ -129,20 +104,6 @@ struct Digits {
     }
 };
 
-// (a, b) += m * (x, y) as packed f32 pairs
-__device__ __forceinline__ void fma2(float (&o)[2], float m, float x, float y) {
-    asm("{\n\t.reg .b64 d, a, b;\n\tmov.b64 d, {%0, %1};\n\tmov.b64 a, {%2, %2};\n\tmov.b64 b, {%3, %4};\n\t"
-        "fma.rn.f32x2 d, a, b, d;\n\tmov.b64 {%0, %1}, d;\n\t}"
-        : "+f"(o[0]), "+f"(o[1])
-        : "f"(m), "f"(x), "f"(y));
-}
-__device__ __forceinline__ void add2(float &x, float &y, float v) {
-    asm("{\n\t.reg .b64 d, a;\n\tmov.b64 d, {%0, %1};\n\tmov.b64 a, {%2, %2};\n\tadd.rn.f32x2 d, d, a;\n\t"
-        "mov.b64 {%0, %1}, d;\n\t}"
-        : "+f"(x), "+f"(y)
-        : "f"(v));
-}
-
 template <int HD, int SLOTS>
 struct DecodeSmem {
     static constexpr int kRow = HD + 8;  // eight rows' stores meet different banks
@@ -155,7 +116,7 @@ struct DecodeSmem {
     float m[kDWarps][SLOTS], l[kDWarps][SLOTS];
     // what the cluster's CTAs send: their outputs for this CTA's share, and (maximum, sum)
     float4 from[SLOTS * HD / 4];
-    float2 ml[kDMaxCluster][SLOTS];
+    float2 ml[kMaxCluster][SLOTS];
 };
 
 // 16 bytes global -> shared, past L1
