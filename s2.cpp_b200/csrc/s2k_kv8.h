@@ -205,6 +205,9 @@ cudaError_t launch_kv8_append(const Kv8 &c, const Kv8Rows &r, const Rows &k, con
 cudaError_t launch_kv8_read(const Kv8 &c, const Kv8Rows &r, const Rows &k, const Rows &v, cudaStream_t st);
 cudaError_t launch_kv8_attend(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, cudaStream_t st);
 
+// the same for calls of many rows per sequence
+cudaError_t launch_kv8_prompt(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, cudaStream_t st);
+
 struct LogprobArgs {
     const void *x = nullptr;
     int type = OT_F32;

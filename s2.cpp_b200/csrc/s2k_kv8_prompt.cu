@@ -1,0 +1,544 @@
+// s2k_kv8_prompt.cu -- attention of many query rows (prompts) over the 8-bit
+// paged KV cache, on the tensor cores (tcgen05).
+//
+// The same sums as s2k_kv8_attn.cu; here a kv head's pages are read for 128 or
+// 256 slots at once (a slot is one (row, query head) pair of the kv head), so
+// the products are the bound: 4 * head_dim operations per slot and visible key
+// at the f16 rate, and one exponential per slot and key, which at 16 per cycle
+// and SM takes as long as the products at head_dim 128 and twice as long at 64.
+//
+// One CTA per tile of slots; a step is 128 keys (8 pages):
+//   warps 8-11   producers: int8 pages -> f16 operands in shared memory, two
+//                steps deep (128-byte swizzled rows, K-major: keys [key][dim],
+//                values [dim][key], which is how the cache holds them).  Every
+//                int8 is exact in f16; the blocks' scales stay apart.
+//   warp 12      one lane issues the products: S = Q K^T (128 x 128, f32 in
+//                TMEM), O += P V with P from TMEM.
+//   warps 0-3, 4-7   two groups of one row per thread: softmax of S, P as f16
+//                over S's own columns, O's factor, the output.
+// The groups take turns: while one forms its weights, the other's products
+// run.  f16 / bf16 rows: 256 slots, 128 per group, every step.  f32 rows, and a
+// last tile of up to 128 slots: both groups have the same 128 slots and take
+// alternate steps, joined at the end.
+//
+// Rounding.  Q is f16 after a power of two per slot (exact for f16 and bf16
+// rows but for elements 2^-28 below the slot's largest).  P is f16, relative to
+// a reference within 2^8 of the running maximum, times the blocks' value scales
+// relative to a power of two above the largest seen: 2^15 at most, f16's full
+// precision down to 2^-29 of that.  f32 rows add what both roundings left over
+// as second f16 operands: twice the products for 22 bits.  Maxima and sums are
+// f32.  O stays in TMEM (f32) and is rescaled only when a reference moves: for a
+// row's first steps and rarely after.
+#include "s2k_common.cuh"
+#include "s2k_kv8.h"
+#include "s2k_tc.cuh"
+
+#include <algorithm>
+#include <atomic>
+
+namespace s2k {
+
+constexpr int kPM = 128;        // slots of a group, keys of a step
+constexpr int kPPages = kPM / kPage;
+constexpr int kPThreads = 13 * 32;
+constexpr int kPMeta = 4;       // steps whose scales and positions are held
+constexpr float kPTop = 128.f;  // a weight at its reference, with the largest value scale
+constexpr float kPSlack = 8.f;  // how far (log2) the running maximum may pass the reference
+constexpr int kPNone = 0x7fffff00;  // "first token" of no page: behind every position
+
+template <int HD>
+struct PromptSmem {
+    static constexpr int NC = HD / 64;
+    alignas(1024) uint8_t q[2][NC][kPM * 128];  // f32: rounded, left over; else the groups'
+    alignas(1024) uint8_t k[2][NC][kPM * 128];
+    alignas(1024) uint8_t v[2][2][HD * 128];
+    float qmul[2][kPM];
+    struct Meta {
+        float ks[kPPages], vs[kPPages];
+        int p0[kPPages];
+    };
+    alignas(16) Meta meta[kPMeta];
+    float join[3][kPM];
+    uint64_t kfull[2], kempty[2], vfull[2], vempty[2], mfull[kPMeta], sfull[2], pfull[2], odone[2];
+    uint32_t tmem;
+};
+
+// kind::f16: D f32, A and B f16, K-major, M = 128
+template <int N>
+constexpr uint32_t prompt_idesc() {
+    return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kPM >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, int acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Four int8 (one word) -> two f16 pairs, exactly: q + 128 in the low bits of
+// 1024's mantissa, minus 1152.
+__device__ __forceinline__ void cvt_i8x4(uint32_t w, uint32_t &a, uint32_t &b) {
+    w ^= 0x80808080u;
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    uint32_t lo = __byte_perm(w, 0x64646464u, 0x4140), hi = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 l = __hsub2(*reinterpret_cast<__half2 *>(&lo), bias);
+    const __half2 h = __hsub2(*reinterpret_cast<__half2 *>(&hi), bias);
+    a = *reinterpret_cast<const uint32_t *>(&l);
+    b = *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t half2_bits(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// what rounding (x, y) to the f16 pair h left over
+__device__ __forceinline__ uint32_t left_over(float x, float y, uint32_t h) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+    return half2_bits(x - f.x, y - f.y);
+}
+// byte offset of 16-byte piece `piece` of row `row` in a 128-byte swizzled operand
+__device__ __forceinline__ int swz(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
+
+template <int HD, int TYPE>
+__global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows r, Kv8Attn a, int vec) {
+    using T = typename OType<TYPE>::T;
+    using Sm = PromptSmem<HD>;
+    constexpr bool wide = TYPE == OT_F32;
+    constexpr int NC = Sm::NC, SLOTS = wide ? kPM : 2 * kPM;
+    constexpr unsigned kAll = 0xffffffffu;
+    extern __shared__ uint8_t raw[];
+    Sm &sm = *reinterpret_cast<Sm *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // later tiles see more keys: they start first
+    const int b = blockIdx.x % r.n_seqs, tile = gridDim.x / r.n_seqs - 1 - blockIdx.x / r.n_seqs, kvh = blockIdx.y;
+    const int G = a.n_heads / c.n_kv_heads;
+    int row0, n, past;
+    if (!kv8_seq(r, b, row0, n, past) || (long long)tile * SLOTS >= (long long)n * G) return;
+    const int slot0 = tile * SLOTS, nslots = (int)min((long long)SLOTS, (long long)n * G - slot0);
+    const bool split = wide || nslots <= kPM;  // the groups share the slots and alternate in steps
+    const int pos_lo = past + slot0 / G, pos_hi = past + (slot0 + nslots - 1) / G;
+    const int wlo = a.window ? max(pos_lo - a.window + 1, 0) : 0;
+    const int fw = wlo / kPage;
+    const int ns = min((int)(((long long)a.sinks + kPage - 1) / kPage), fw);
+    const int total = ns + pos_hi / kPage - fw + 1;
+    const int steps = (total + kPPages - 1) / kPPages;
+    const int jobs = split ? steps : 2 * steps;  // job g: group g % 2, step g or g / 2
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sm.kfull[i], 4);
+            mbar_init(&sm.vfull[i], 4);
+            mbar_init(&sm.kempty[i], 1);
+            mbar_init(&sm.vempty[i], 1);
+            mbar_init(&sm.sfull[i], 1);
+            mbar_init(&sm.pfull[i], kPM);
+            mbar_init(&sm.odone[i], 1);
+        }
+        for (int i = 0; i < kPMeta; ++i) mbar_init(&sm.mfull[i], 4);
+        fence_mbar_init();
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // queries -> f16 operands, a warp a slot at a time
+    if (warp < 8) {
+        constexpr int E = HD / 32;
+        const float sign = a.scale < 0.f ? -1.f : 1.f;
+        const int half = nslots > kPM ? 2 * kPM : kPM;
+        for (int s = warp; s < half; s += 8) {
+            const int st = slot0 + min(s, nslots - 1), row = st / G;
+            float x[E];
+            load_n<E>(reinterpret_cast<const T *>(a.q.p) + (long long)(row0 + row) * a.q.row_stride +
+                          (long long)(kvh * G + st - row * G) * a.q.head_stride + lane * E,
+                      vec, x);
+            unsigned top = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+            top = __reduce_max_sync(kAll, top);
+            // 2^-e brings the slot's largest to 2^13 .. 2^14
+            const int e2 = max((int)(top >> 23) - 127, -112) - 13;
+            const float down = sign * __int_as_float((127 - e2) << 23);
+            if (lane == 0)
+                sm.qmul[s / kPM][s % kPM] =
+                    top >= 0x7f800000u ? NAN : fabsf(a.scale) * 1.44269504f * __int_as_float((e2 + 127) << 23);
+            uint32_t h[E / 2], lo[E / 2];
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e) {
+                h[e] = half2_bits(x[2 * e] * down, x[2 * e + 1] * down);
+                lo[e] = wide ? left_over(x[2 * e] * down, x[2 * e + 1] * down, h[e]) : 0;
+            }
+            const int dim = lane * E, at = swz(s % kPM, dim % 64 / 8) + dim % 8 * 2;
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e) {
+                *reinterpret_cast<uint32_t *>(&sm.q[s / kPM][dim / 64][at + 4 * e]) = h[e];
+                if (wide) *reinterpret_cast<uint32_t *>(&sm.q[1][dim / 64][at + 4 * e]) = lo[e];
+            }
+        }
+        fence_proxy_async_smem();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem;
+    bool ok = true;
+
+    if (warp >= 8 && warp < 12) {
+        // ---------------- producers: two pages of each step per warp ----------------
+        const int pw = warp - 8;
+        constexpr int U = HD / 32;  // 16-byte pieces per lane and page
+        uint4 kr[2][U], vr[2][U];
+        auto pages_of = [&](int t, int (&pg)[2]) {  // lanes 0 and 1 look them up
+            const int x = t * kPPages + 2 * pw + (lane & 1);
+            const int lg = x < ns ? x : x - ns + fw;
+            const int p = t < steps && x < total && lane < 2 ? kv8_page(c, r, b, lg) : -1;
+            pg[0] = __shfl_sync(kAll, p, 0);
+            pg[1] = __shfl_sync(kAll, p, 1);
+        };
+        auto fetch = [&](const int8_t *src, const int (&pg)[2], uint4 (&x)[2][U]) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    x[e][u] = pg[e] >= 0 ? *reinterpret_cast<const uint4 *>(src + c.block(pg[e], kvh) * (kPage * HD) +
+                                                                          (u * 32 + lane) * 16)
+                                         : make_uint4(0, 0, 0, 0);
+        };
+        auto put = [&](uint8_t *buf, int row, int piece, uint32_t w0, uint32_t w1) {
+            uint4 h;
+            cvt_i8x4(w0, h.x, h.y);
+            cvt_i8x4(w1, h.z, h.w);
+            *reinterpret_cast<uint4 *>(buf + swz(row, piece)) = h;
+        };
+        int pg[2], pn[2];
+        pages_of(0, pg);
+        fetch(c.k, pg, kr);
+        for (int t = 0; t < steps && ok; ++t) {
+            const int s = t & 1;
+            fetch(c.v, pg, vr);
+            pages_of(t + 1, pn);
+            if (t >= 2) ok = mbar_wait(&sm.kempty[s], ((t >> 1) - 1) & 1, r.err, ERR_WAIT_EMPTY);
+            if (!(ok = __all_sync(kAll, ok))) break;
+            if (lane < 2) {
+                typename Sm::Meta &m = sm.meta[t % kPMeta];
+                const int i = 2 * pw + lane, p = lane ? pg[1] : pg[0], x = t * kPPages + i;
+                m.ks[i] = p >= 0 ? c.k_scale[c.block(p, kvh)] : 0.f;
+                m.vs[i] = p >= 0 ? c.v_scale[c.block(p, kvh)] : 0.f;
+                m.p0[i] = p >= 0 ? (x < ns ? x : x - ns + fw) * kPage : kPNone;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.mfull[t % kPMeta]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    // piece x of a key's 16-dim pieces; lanes of the upper 64 dims store their halves in the other
+                    // order, so that eight lanes meet all banks
+                    const int id = u * 32 + lane, row = (2 * pw + e) * kPage + id / (HD / 16), x = id % (HD / 16);
+                    uint8_t *buf = sm.k[s][x / 4];
+                    const int flip = x / 4 & 1;
+                    const uint4 w = kr[e][u];
+                    put(buf, row, 2 * (x % 4) + flip, flip ? w.z : w.x, flip ? w.w : w.y);
+                    put(buf, row, 2 * (x % 4) + 1 - flip, flip ? w.x : w.z, flip ? w.y : w.w);
+                }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.kfull[s]);
+            fetch(c.k, pn, kr);
+            if (t >= 2) ok = mbar_wait(&sm.vempty[s], ((t >> 1) - 1) & 1, r.err, ERR_WAIT_EMPTY);
+            if (!(ok = __all_sync(kAll, ok))) break;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int d = u * 32 + lane, page = 2 * pw + e;
+                    uint8_t *buf = sm.v[s][page / 4];
+                    const uint4 w = vr[e][u];
+                    put(buf, d, 2 * (page % 4), w.x, w.y);
+                    put(buf, d, 2 * (page % 4) + 1, w.z, w.w);
+                }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.vfull[s]);
+            pg[0] = pn[0], pg[1] = pn[1];
+        }
+    } else if (warp == 12) {
+        // ---------------- products ----------------
+        if (lane == 0) {
+            auto qk = [&](int g) {
+                const int t = split ? g : g >> 1, w = g & 1, s = t & 1;
+                if (!mbar_wait(&sm.kfull[s], (t >> 1) & 1, r.err, ERR_WAIT_FULL)) return false;
+                tc_fence_after();
+                const uint32_t d = tmem + w * kPM;
+#pragma unroll
+                for (int x = 0; x < 4 * NC; ++x)
+                    mma_ss(d, sw128_desc(&sm.q[split ? 0 : w][x / 4][32 * (x % 4)]), sw128_desc(&sm.k[s][x / 4][32 * (x % 4)]),
+                           prompt_idesc<kPM>(), x != 0);
+                if (wide) {
+#pragma unroll
+                    for (int x = 0; x < 4 * NC; ++x)
+                        mma_ss(d, sw128_desc(&sm.q[1][x / 4][32 * (x % 4)]), sw128_desc(&sm.k[s][x / 4][32 * (x % 4)]),
+                               prompt_idesc<kPM>(), 1);
+                }
+                mma_commit(&sm.sfull[w]);
+                if (split || w) mma_commit(&sm.kempty[s]);
+                return true;
+            };
+            ok = qk(0);
+            if (ok && jobs > 1) ok = qk(1);
+            for (int g = 0; g < jobs && ok; ++g) {
+                const int t = split ? g : g >> 1, w = g & 1, s = t & 1;
+                if (!(ok = mbar_wait(&sm.pfull[w], (g >> 1) & 1, r.err, ERR_WAIT_FULL))) break;
+                if (!(ok = mbar_wait(&sm.vfull[s], (t >> 1) & 1, r.err, ERR_WAIT_FULL))) break;
+                tc_fence_after();
+                const uint32_t d = tmem + 2 * kPM + w * kPM, p = tmem + w * kPM;
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {  // 16 keys each
+                    const uint64_t v = sw128_desc(&sm.v[s][x / 4][32 * (x % 4)]);
+                    mma_ts(d, p + 32 * (x / 2) + 8 * (x % 2), v, prompt_idesc<HD>(), g > 1 || x > 0);
+                    if (wide) mma_ts(d, p + 32 * (x / 2) + 16 + 8 * (x % 2), v, prompt_idesc<HD>(), 1);
+                }
+                if (split || w) mma_commit(&sm.vempty[s]);
+                if (g + 2 >= jobs) mma_commit(&sm.odone[w]);
+                if (g + 2 < jobs) ok = qk(g + 2);
+            }
+        }
+    } else {
+        // ---------------- softmax: one row per thread ----------------
+        const int w = warp >> 2, row = tid & (kPM - 1), ls = (split ? 0 : w * kPM) + row;
+        const int st = slot0 + min(ls, nslots - 1), ti = st / G;
+        const int pos = past + ti;
+        // positions of the warp's rows
+        const int s_lo = slot0 + min(ls - lane, nslots - 1), s_hi = slot0 + min(ls - lane + 31, nslots - 1);
+        const int p_min = past + s_lo / G, p_max = past + s_hi / G;
+        const float smul = sm.qmul[split ? 0 : w][row];
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t S = tmem + lanes + w * kPM, O = tmem + lanes + 2 * kPM + w * kPM;
+        float ref = -INFINITY, l = 0.f, vref = 7.8886090522101181e-31f;
+        int done = 0;  // this group's jobs so far
+        for (int g = w; g < jobs && ok; g += 2, ++done) {
+            const int t = split ? g : g >> 1;
+            ok = mbar_wait(&sm.mfull[t % kPMeta], (t / kPMeta) & 1, r.err, ERR_WAIT_FULL) &&
+                 mbar_wait(&sm.sfull[w], done & 1, r.err, ERR_WAIT_FULL);
+            if (!(ok = __all_sync(kAll, ok))) break;
+            tc_fence_after();
+            const typename Sm::Meta &m = sm.meta[t % kPMeta];
+            int lo = m.p0[0], hi = m.p0[0];
+            float vmax = m.vs[0];  // of the blocks that the row sees: its weights' resolution goes by them
+#pragma unroll
+            for (int i = 1; i < kPPages; ++i) {
+                lo = min(lo, m.p0[i]);
+                hi = max(hi, m.p0[i]);
+                vmax = fmaxf(vmax, m.vs[i]);
+            }
+            const bool edge = hi + kPage - 1 > p_min || (a.window && lo <= p_max - a.window && hi + kPage > a.sinks);
+            auto hidden = [&](int j) { return j > pos || (a.window && j <= pos - a.window && j >= a.sinks); };
+            if (edge) {
+                vmax = 0.f;
+#pragma unroll
+                for (int i = 0; i < kPPages; ++i) {
+                    const int p0 = m.p0[i];
+                    if (p0 <= pos && (!a.window || p0 + kPage - 1 > pos - a.window || p0 < a.sinks))
+                        vmax = fmaxf(vmax, m.vs[i]);
+                }
+            }
+            // the step's largest score
+            float mx = -INFINITY;
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch) {
+                int x[32];
+                tmem_ld32(S + 32 * ch, x);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float ks = m.ks[2 * ch + e] * smul;
+                    float top = -INFINITY;
+                    if (edge) {
+                        const int p0 = m.p0[2 * ch + e];
+#pragma unroll
+                        for (int i = 0; i < kPage; ++i)
+                            top = fmaxf(top, hidden(p0 + i) ? -INFINITY : __int_as_float(x[16 * e + i]) * ks);
+                        mx = fmaxf(mx, top);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < kPage; ++i) top = fmaxf(top, __int_as_float(x[16 * e + i]));
+                        mx = fmaxf(mx, top * ks);
+                    }
+                }
+            }
+            const bool far = mx > ref + kPSlack;  // true for the first finite one
+            if (__any_sync(kAll, far || vmax > vref)) {
+                const float r2 = far ? mx : ref;
+                // a power of two from vmax on
+                const float v2 = vmax > vref ? __uint_as_float((__float_as_uint(vmax) + 0x7fffffu) & 0x7f800000u) : vref;
+                const float fl = ref == r2 ? 1.f : ex2(ref - r2), f = fl * (vref / v2);
+                l *= fl;
+                if (done) {
+#pragma unroll
+                    for (int ch = 0; ch < HD / 16; ++ch) {
+                        int x[16];
+                        uint32_t y[16];
+                        tmem_ld16(O + 16 * ch, x);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__int_as_float(x[i]) * f);
+                        tmem_st16(O + 16 * ch, y);
+                    }
+                }
+                ref = r2;
+                vref = v2;
+            }
+            const float base = ref == -INFINITY ? 0.f : ref;
+            const float vmul = kPTop / vref;
+            float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch) {
+                int x[32];
+                uint32_t hi16[16], lo16[16];
+                tmem_ld32(S + 32 * ch, x);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float ks = m.ks[2 * ch + e] * smul, vs = m.vs[2 * ch + e] * vmul;
+                    const int p0 = m.p0[2 * ch + e];
+#pragma unroll
+                    for (int i = 0; i < kPage; i += 2) {
+                        float p = ex2(fmaf(__int_as_float(x[16 * e + i]), ks, -base));
+                        float u = ex2(fmaf(__int_as_float(x[16 * e + i + 1]), ks, -base));
+                        float pv = p * vs, uv = u * vs;
+                        if (edge) {  // a hidden block's scales may be NaN
+                            if (hidden(p0 + i)) p = pv = 0.f;
+                            if (hidden(p0 + i + 1)) u = uv = 0.f;
+                        }
+                        l0 += p;
+                        l1 += u;
+                        hi16[8 * e + i / 2] = half2_bits(pv, uv);
+                        if (wide) lo16[8 * e + i / 2] = left_over(pv, uv, hi16[8 * e + i / 2]);
+                    }
+                }
+                tmem_st16(S + 32 * ch, hi16);
+                if (wide) tmem_st16(S + 32 * ch + 16, lo16);
+            }
+            l += l0 + l1;
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&sm.pfull[w]);
+        }
+        if (ok && done) ok = mbar_wait(&sm.odone[w], 0, r.err, ERR_WAIT_FULL);
+        if (ok && split && w) ok = mbar_wait(&sm.odone[0], 0, r.err, ERR_WAIT_FULL);  // it stores where V was
+        ok = __all_sync(kAll, ok);
+        if (!ok) l = NAN;  // a wait ran out: the result says so
+        tc_fence_after();
+        float f = done ? vref * (1.f / kPTop) : 0.f;  // takes O to sums of weight * value
+        float *xch = reinterpret_cast<float *>(sm.k);  // [kPM][HD + 4], over K and V
+        if (split) {
+            if (w == 1) {
+#pragma unroll
+                for (int ch = 0; ch < HD / 16; ++ch) {
+                    int x[16];
+                    if (done) tmem_ld16(O + 16 * ch, x);
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4)
+                        *reinterpret_cast<float4 *>(&xch[row * (HD + 4) + 16 * ch + i]) =
+                            done ? make_float4(__int_as_float(x[i]) * f, __int_as_float(x[i + 1]) * f,
+                                               __int_as_float(x[i + 2]) * f, __int_as_float(x[i + 3]) * f)
+                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                sm.join[0][row] = ref;
+                sm.join[1][row] = l;
+            }
+            named_sync(1, 2 * kPM);
+        }
+        if ((!split || w == 0) && ls - lane < nslots) {
+            float g1 = 0.f;
+            if (split) {
+                const float ref1 = sm.join[0][row], top = fmaxf(ref, ref1);
+                const float g0 = ref == -INFINITY ? 0.f : ex2(ref - top);
+                g1 = ref1 == -INFINITY ? 0.f : ex2(ref1 - top);
+                l = g0 * l + g1 * sm.join[1][row];
+                f *= g0;
+            }
+            const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+            T *y = reinterpret_cast<T *>(a.out.p) + (long long)(row0 + ti) * a.out.row_stride +
+                   (long long)(kvh * G + st - ti * G) * a.out.head_stride;
+#pragma unroll
+            for (int ch = 0; ch < HD / 16; ++ch) {
+                int x[16];
+                tmem_ld16(O + 16 * ch, x);
+                if (ls < nslots) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        float z[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) z[e] = __int_as_float(x[i + e]) * f;
+                        if (split) {
+                            const float4 o1 = *reinterpret_cast<const float4 *>(&xch[row * (HD + 4) + 16 * ch + i]);
+                            z[0] += g1 * o1.x, z[1] += g1 * o1.y, z[2] += g1 * o1.z, z[3] += g1 * o1.w;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) z[e] *= inv;
+                        store_n<4>(y + 16 * ch + i, vec, z);
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// More than half of an SM's: a CTA holds all of its TMEM, a second one would only wait for it.
+template <int HD>
+constexpr int prompt_smem() {
+    return std::max((int)sizeof(PromptSmem<HD>) + 1024, 120 * 1024);
+}
+
+static std::atomic<int> g_prompt_ready[64];
+
+cudaError_t launch_kv8_prompt(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, cudaStream_t st) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64) return cudaErrorInvalidDevice;
+    if (!g_prompt_ready[dev].load(std::memory_order_acquire)) {
+        for (int hd : {64, 128})
+            for (int type : {OT_F32, OT_F16, OT_BF16})
+                if ((e = kv8_dispatch(hd, type, [&](auto h, auto t) {
+                         return cudaFuncSetAttribute(kv8_prompt_kernel<h, t>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                     prompt_smem<h>());
+                     })))
+                    return e;
+        g_prompt_ready[dev].store(1, std::memory_order_release);
+    }
+    const long long slots = (long long)r.max_rows * (a.n_heads / c.n_kv_heads);
+    const int per = a.q.type == OT_F32 ? kPM : 2 * kPM;
+    const long long tiles = (slots + per - 1) / per;
+    if (slots > 0x7fffffffLL || tiles * r.n_seqs > 0x7fffffffLL) return cudaErrorInvalidValue;
+    const dim3 grid((unsigned)(tiles * r.n_seqs), c.n_kv_heads);
+    const int vec = rows_vec(a.q, 4) && rows_vec(a.out, 4);
+    count_launch();
+    return kv8_dispatch(c.head_dim, a.q.type, [&](auto h, auto t) {
+        kv8_prompt_kernel<h, t><<<grid, kPThreads, prompt_smem<h>(), st>>>(c, r, a, vec);
+        return cudaGetLastError();
+    });
+}
+
+}  // namespace s2k

@@ -68,12 +68,13 @@ def seen(pos, n, window, sinks):
 def attend(k, v, q, past, scale, window=0, sinks=0, vtop=None):
     """One sequence: k, v [n][Hkv][dim], q [T][H][dim] at positions past...  Returns out [T][H][dim]; the summed
     |weight * value| [T][H][dim]; each row's largest scale * sum |q k| (the scores' size); its largest scale * max|q| *
-    sum |k|; and the sum over pages of 2 * 32 * (the page's largest weight * vtop), vtop [n][Hkv] what a position's
-    block can hold at most (a pair's largest is at most the sum of its two pages', twice for either pairing)."""
+    sum |k|; the sum over pages of 2 * 32 * (the page's largest weight * vtop), vtop [n][Hkv] what a position's block
+    can hold at most (a pair's largest is at most the sum of its two pages', twice for either pairing); and the
+    number of keys * the largest weight * the largest vtop."""
     T, H, D = q.shape
     G = H // k.shape[1]
     out, mag = np.zeros((T, H, D)), np.zeros((T, H, D))
-    size, reach, grain = np.zeros((T, H)), np.zeros((T, H)), np.zeros((T, H))
+    size, reach, grain, coarse = np.zeros((4, T, H))
     for i in range(T):
         m = seen(past + i, k.shape[0], window, sinks)
         if not m.any():
@@ -91,4 +92,5 @@ def attend(k, v, q, past, scale, window=0, sinks=0, vtop=None):
                 x = np.zeros((k.shape[0] + PAGE - 1) // PAGE * PAGE)
                 x[: k.shape[0]][m] = w * vtop[m, h // G]
                 grain[i, h] = 64 * x.reshape(-1, PAGE).max(1).sum()
-    return out, mag, size, reach, grain
+                coarse[i, h] = len(w) * w.max() * vtop[m, h // G].max()
+    return out, mag, size, reach, grain, coarse

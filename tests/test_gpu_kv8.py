@@ -13,7 +13,11 @@ that; the weights' rounding to f16 in the prompt kernel adds 2^-11 twice
 Weights are held in fixed point relative to the largest of their pair of pages
 (32 keys): to 2^-16 of it for 16-bit rows, 2^-30 for f32 ones, whatever their
 own size; for the 32 keys together 32 * that * (the pair's largest weight times
-value scale) * 127, which `grain` sums over all pairs (of either parity).
+value scale) * 127, which `grain` sums over all pairs (of either parity).  The
+prompt kernel's weights are f16 (f32 rows: and what that left over) with the
+largest weight times the largest value scale at 2^7 or up to twice above: f16's
+unit below 2^-14 is 2^-24, so a weight is off by up to 2^-25 / 2^6 of that,
+2^-31 times `coarse` for all keys together.
 """
 from __future__ import annotations
 
@@ -81,9 +85,9 @@ class Call:
             v = ku.values(self.vq, self.vs, self.layer, self.table[b], p + t, True)
             sl = slice(self.start[b], self.start[b + 1])
             vtop = np.repeat(self.vs[self.table[b, : (p + t + 15) // 16], self.layer].astype(np.float64), 16, 0)[: p + t] * 127
-            want, mag, size, reach, grain = ku.attend(k, v, qn[sl], p, scale, window, sinks, vtop)
+            want, mag, size, reach, grain, coarse = ku.attend(k, v, qn[sl], p, scale, window, sinks, vtop)
             score = 2.0**-20 * size + QUERY[self.typ] * reach
-            tol = GRAIN[self.typ] * grain[..., None] + mag * (2 * score[..., None] + EXTRA[self.typ]) + np.abs(want) * HALF_STEP[self.typ] * 1.01 + 1e-30
+            tol = (GRAIN[self.typ] * grain + 2.0**-31 * coarse)[..., None] + mag * (2 * score[..., None] + EXTRA[self.typ]) + np.abs(want) * HALF_STEP[self.typ] * 1.01 + 1e-30
             d = np.abs(on[sl] - want)
             assert np.all(d <= tol), f"sequence {b}: {np.nanmax(d / tol)} times the tolerance"
 
@@ -295,7 +299,7 @@ def test_far_pages_pass_32_bit_offsets():
     q = torch.randn(40, 4, D, device="cuda")
     out = cache.attend(0, q, i32([0]), table)
     one = cache.attend(0, q[39:], i32([39]), table)
-    want, mag, size, _, _ = ku.attend(kb.double().cpu().numpy(), vb.double().cpu().numpy(), q.double().cpu().numpy(), 0, D ** -0.5)
+    want, mag, size, _, _, _ = ku.attend(kb.double().cpu().numpy(), vb.double().cpu().numpy(), q.double().cpu().numpy(), 0, D ** -0.5)
     tol = mag * (2 * 2.0**-20 * size[..., None] + EXTRA["f32"]) + np.abs(want) * 2.0**-24 * 2
     assert np.all(np.abs(out.double().cpu().numpy() - want) <= tol)
     assert np.all(np.abs(one[0].double().cpu().numpy() - want[39]) <= tol[39])
