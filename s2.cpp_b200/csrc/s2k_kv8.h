@@ -135,6 +135,12 @@ __device__ __forceinline__ void fma2(float (&o)[2], float m, float x, float y) {
         : "+f"(o[0]), "+f"(o[1])
         : "f"(m), "f"(x), "f"(y));
 }
+__device__ __forceinline__ void mul2(float (&o)[2], float m) {
+    asm("{\n\t.reg .b64 d, a;\n\tmov.b64 d, {%0, %1};\n\tmov.b64 a, {%2, %2};\n\tmul.rn.f32x2 d, d, a;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "+f"(o[0]), "+f"(o[1])
+        : "f"(m));
+}
 __device__ __forceinline__ void add2(float &x, float &y, float v) {
     asm("{\n\t.reg .b64 d, a;\n\tmov.b64 d, {%0, %1};\n\tmov.b64 a, {%2, %2};\n\tadd.rn.f32x2 d, d, a;\n\t"
         "mov.b64 {%0, %1}, d;\n\t}"

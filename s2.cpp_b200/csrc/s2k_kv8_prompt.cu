@@ -15,20 +15,24 @@
 //   warp 12      one lane issues the products: S = Q K^T (128 x 128, f32 in
 //                TMEM), O += P V with P from TMEM.
 //   warps 0-3, 4-7   two groups of one row per thread: softmax of S, P as f16
-//                over S's own columns, O's factor, the output.
+//                over S's own columns, the output.
 // The groups take turns: while one forms its weights, the other's products
-// run.  f16 / bf16 rows: 256 slots, 128 per group, every step.  f32 rows, and a
-// last tile of up to 128 slots: both groups have the same 128 slots and take
-// alternate steps, joined at the end.
+// run.  f16 / bf16 rows: 256 slots, 128 per group, every step.  A last tile of
+// up to 128 slots, and f32 rows: both groups have the same 128 slots and take
+// alternate steps.
 //
-// Rounding.  Q is f16 after a power of two per slot (exact for f16 and bf16
-// rows but for elements 2^-28 below the slot's largest).  P is f16, relative to
-// a reference within 2^8 of the running maximum, times the blocks' value scales
+// Rounding, f16 / bf16 rows.  Q is f16 after a power of two per slot (exact but
+// for elements 2^-28 below the slot's largest).  P is f16, relative to a
+// reference within 2^8 of the running maximum, times the blocks' value scales
 // relative to a power of two above the largest seen: 2^15 at most, f16's full
-// precision down to 2^-29 of that.  f32 rows add what both roundings left over
-// as second f16 operands: twice the products for 22 bits.  Maxima and sums are
-// f32.  O stays in TMEM (f32) and is rescaled only when a reference moves: for a
-// row's first steps and rarely after.
+// precision down to 2^-29 of that.  O stays in TMEM (f32) and is rescaled only
+// when a reference moves: in a row's first steps and rarely after.
+//
+// f32 rows.  Q and P are two f16 operands each, rounded and left over: twice the
+// products for 22 bits.  Sums in TMEM lose a little at every addition (they are
+// cut, not rounded), which over a long context would show in f32: each step's
+// O is taken out and added in registers, half of the dimensions by each group,
+// with the step's own maximum and value scale as its reference.
 #include "s2k_common.cuh"
 #include "s2k_kv8.h"
 #include "s2k_tc.cuh"
@@ -40,9 +44,10 @@ namespace s2k {
 
 constexpr int kPM = 128;        // slots of a group, keys of a step
 constexpr int kPPages = kPM / kPage;
-constexpr int kPThreads = 13 * 32;
+constexpr int kPThreads = 512;  // warps 13-15 only make the register shares whole groups of four warps
 constexpr int kPMeta = 4;       // steps whose scales and positions are held
 constexpr float kPTop = 128.f;  // a weight at its reference, with the largest value scale
+constexpr float kPStepTop = 16384.f;  // the same for f32 rows, whose reference is the step's maximum
 constexpr float kPSlack = 8.f;  // how far (log2) the running maximum may pass the reference
 constexpr int kPNone = 0x7fffff00;  // "first token" of no page: behind every position
 
@@ -58,8 +63,10 @@ struct PromptSmem {
         int p0[kPPages];
     };
     alignas(16) Meta meta[kPMeta];
-    float join[3][kPM];
-    uint64_t kfull[2], kempty[2], vfull[2], vempty[2], mfull[kPMeta], sfull[2], pfull[2], odone[2];
+    float join[2][kPM];
+    float4 stat[kPMeta][kPM];  // f32 rows: a step's reference, sum and what an O of 1 is worth
+    uint64_t kfull[2], kempty[2], vfull[2], vempty[2], mfull[kPMeta], sfull[2], pfull[2][2], odone[2];
+    uint64_t tfull[kPMeta], ofree[2];
     uint32_t tmem;
 };
 
@@ -147,10 +154,15 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             mbar_init(&sm.kempty[i], 1);
             mbar_init(&sm.vempty[i], 1);
             mbar_init(&sm.sfull[i], 1);
-            mbar_init(&sm.pfull[i], kPM);
+            mbar_init(&sm.pfull[i][0], kPM);
+            mbar_init(&sm.pfull[i][1], kPM);
             mbar_init(&sm.odone[i], 1);
+            mbar_init(&sm.ofree[i], 2 * kPM);
         }
-        for (int i = 0; i < kPMeta; ++i) mbar_init(&sm.mfull[i], 4);
+        for (int i = 0; i < kPMeta; ++i) {
+            mbar_init(&sm.mfull[i], 4);
+            mbar_init(&sm.tfull[i], kPM);
+        }
         fence_mbar_init();
     }
     if (warp == 12) {
@@ -200,8 +212,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
     const uint32_t tmem = sm.tmem;
     bool ok = true;
 
+    // registers: 512 threads start with 128 each, and 2 * 168 + 96 + 72 <= 4 * 128
     if (warp >= 8 && warp < 12) {
         // ---------------- producers: two pages of each step per warp ----------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
         const int pw = warp - 8;
         constexpr int U = HD / 32;  // 16-byte pieces per lane and page
         uint4 kr[2][U], vr[2][U];
@@ -279,23 +293,24 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             if (lane == 0) mbar_arrive(&sm.vfull[s]);
             pg[0] = pn[0], pg[1] = pn[1];
         }
-    } else if (warp == 12) {
+    } else if (warp >= 12) {
         // ---------------- products ----------------
-        if (lane == 0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 12 && lane == 0) {
+            // an operand's next 16 columns of K are 32 bytes on, the next 64 a chunk
+            const uint64_t q0 = sw128_desc(sm.q[0][0]), q1 = sw128_desc(sm.q[1][0]);
+            auto at = [](int x, int chunk) { return (uint64_t)(2 * (x % 4) + (x / 4) * (chunk >> 4)); };
             auto qk = [&](int g) {
                 const int t = split ? g : g >> 1, w = g & 1, s = t & 1;
                 if (!mbar_wait(&sm.kfull[s], (t >> 1) & 1, r.err, ERR_WAIT_FULL)) return false;
                 tc_fence_after();
                 const uint32_t d = tmem + w * kPM;
-#pragma unroll
-                for (int x = 0; x < 4 * NC; ++x)
-                    mma_ss(d, sw128_desc(&sm.q[split ? 0 : w][x / 4][32 * (x % 4)]), sw128_desc(&sm.k[s][x / 4][32 * (x % 4)]),
-                           prompt_idesc<kPM>(), x != 0);
+                const uint64_t q = !split && w ? q1 : q0, k = sw128_desc(sm.k[s][0]);
+#pragma unroll 2
+                for (int x = 0; x < 4 * NC; ++x) mma_ss(d, q + at(x, kPM * 128), k + at(x, kPM * 128), prompt_idesc<kPM>(), x != 0);
                 if (wide) {
-#pragma unroll
-                    for (int x = 0; x < 4 * NC; ++x)
-                        mma_ss(d, sw128_desc(&sm.q[1][x / 4][32 * (x % 4)]), sw128_desc(&sm.k[s][x / 4][32 * (x % 4)]),
-                               prompt_idesc<kPM>(), 1);
+#pragma unroll 2
+                    for (int x = 0; x < 4 * NC; ++x) mma_ss(d, q1 + at(x, kPM * 128), k + at(x, kPM * 128), prompt_idesc<kPM>(), 1);
                 }
                 mma_commit(&sm.sfull[w]);
                 if (split || w) mma_commit(&sm.kempty[s]);
@@ -305,23 +320,31 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             if (ok && jobs > 1) ok = qk(1);
             for (int g = 0; g < jobs && ok; ++g) {
                 const int t = split ? g : g >> 1, w = g & 1, s = t & 1;
-                if (!(ok = mbar_wait(&sm.pfull[w], (g >> 1) & 1, r.err, ERR_WAIT_FULL))) break;
-                if (!(ok = mbar_wait(&sm.vfull[s], (t >> 1) & 1, r.err, ERR_WAIT_FULL))) break;
-                tc_fence_after();
                 const uint32_t d = tmem + 2 * kPM + w * kPM, p = tmem + w * kPM;
-#pragma unroll
-                for (int x = 0; x < 8; ++x) {  // 16 keys each
-                    const uint64_t v = sw128_desc(&sm.v[s][x / 4][32 * (x % 4)]);
-                    mma_ts(d, p + 32 * (x / 2) + 8 * (x % 2), v, prompt_idesc<HD>(), g > 1 || x > 0);
-                    if (wide) mma_ts(d, p + 32 * (x / 2) + 16 + 8 * (x % 2), v, prompt_idesc<HD>(), 1);
+                const uint64_t v = sw128_desc(sm.v[s][0]);
+                ok = mbar_wait(&sm.vfull[s], (t >> 1) & 1, r.err, ERR_WAIT_FULL);
+                // f32 rows: the output of two steps ago has been taken
+                if (ok && wide && g > 1) ok = mbar_wait(&sm.ofree[w], ((g >> 1) - 1) & 1, r.err, ERR_WAIT_EMPTY);
+                for (int h = 0; h < 2 && ok; ++h) {  // 64 keys each
+                    if (!(ok = mbar_wait(&sm.pfull[w][h], (g >> 1) & 1, r.err, ERR_WAIT_FULL))) break;
+                    tc_fence_after();
+#pragma unroll 2
+                    for (int y = 0; y < 4; ++y) {
+                        const uint64_t vx = v + at(y, 0) + h * (HD * 128 >> 4);
+                        const uint32_t px = p + 64 * h + 32 * (y / 2) + 8 * (y % 2);
+                        mma_ts(d, px, vx, prompt_idesc<HD>(), (!wide && g > 1) || h > 0 || y > 0);
+                        if (wide) mma_ts(d, px + 16, vx, prompt_idesc<HD>(), 1);
+                    }
                 }
+                if (!ok) break;
                 if (split || w) mma_commit(&sm.vempty[s]);
-                if (g + 2 >= jobs) mma_commit(&sm.odone[w]);
+                if (wide || g + 2 >= jobs) mma_commit(&sm.odone[w]);
                 if (g + 2 < jobs) ok = qk(g + 2);
             }
         }
     } else {
         // ---------------- softmax: one row per thread ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
         const int w = warp >> 2, row = tid & (kPM - 1), ls = (split ? 0 : w * kPM) + row;
         const int st = slot0 + min(ls, nslots - 1), ti = st / G;
         const int pos = past + ti;
@@ -332,8 +355,42 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t S = tmem + lanes + w * kPM, O = tmem + lanes + 2 * kPM + w * kPM;
         float ref = -INFINITY, l = 0.f, vref = 7.8886090522101181e-31f;
+        // f32 rows: this group's half of the output
+        constexpr int HALF = wide ? HD / 2 : 1;
+        float acc[HALF];
+#pragma unroll
+        for (int i = 0; i < HALF; ++i) acc[i] = 0.f;
+        float top_ref = -INFINITY, sum = 0.f;
+        auto take = [&](int t) {  // f32 rows: adds step t's output
+            bool fine = mbar_wait(&sm.tfull[t % kPMeta], (t / kPMeta) & 1, r.err, ERR_WAIT_FULL) &&
+                        mbar_wait(&sm.odone[t & 1], (t >> 1) & 1, r.err, ERR_WAIT_FULL);
+            if (!__all_sync(kAll, fine)) return false;
+            tc_fence_after();
+            const float4 z = sm.stat[t % kPMeta][row];
+            const float r2 = fmaxf(top_ref, z.x);
+            const float f0 = top_ref == r2 ? 1.f : ex2(top_ref - r2), f1 = z.x == -INFINITY ? 0.f : ex2(z.x - r2);
+            const float mul = f1 * z.z;
+            sum = sum * f0 + z.y * f1;
+            top_ref = r2;
+            const uint32_t from = tmem + lanes + 2 * kPM + (t & 1) * kPM + w * HALF;
+#pragma unroll
+            for (int ch = 0; ch < (HALF + 15) / 16; ++ch) {
+                int x[16];
+                tmem_ld16(from + 16 * ch, x);
+#pragma unroll
+                for (int i = 0; i < 16 && 16 * ch + i < HALF; ++i)
+                    acc[16 * ch + i] = fmaf(mul, __int_as_float(x[i]), acc[16 * ch + i] * f0);
+            }
+            tc_fence_before();
+            mbar_arrive(&sm.ofree[t & 1]);
+            return true;
+        };
         int done = 0;  // this group's jobs so far
-        for (int g = w; g < jobs && ok; g += 2, ++done) {
+        for (int g = wide ? 0 : w; g < jobs && ok; g += wide ? 1 : 2) {
+            if (wide && (g & 1) != w) {  // the other group's step
+                if (g > 0) ok = take(g - 1);
+                continue;
+            }
             const int t = split ? g : g >> 1;
             ok = mbar_wait(&sm.mfull[t % kPMeta], (t / kPMeta) & 1, r.err, ERR_WAIT_FULL) &&
                  mbar_wait(&sm.sfull[w], done & 1, r.err, ERR_WAIT_FULL);
@@ -349,149 +406,198 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 vmax = fmaxf(vmax, m.vs[i]);
             }
             const bool edge = hi + kPage - 1 > p_min || (a.window && lo <= p_max - a.window && hi + kPage > a.sinks);
-            auto hidden = [&](int j) { return j > pos || (a.window && j <= pos - a.window && j >= a.sinks); };
-            if (edge) {
-                vmax = 0.f;
-#pragma unroll
-                for (int i = 0; i < kPPages; ++i) {
-                    const int p0 = m.p0[i];
-                    if (p0 <= pos && (!a.window || p0 + kPage - 1 > pos - a.window || p0 < a.sinks))
-                        vmax = fmaxf(vmax, m.vs[i]);
-                }
-            }
-            // the step's largest score
+            // bit i: the row sees token i of page pg
+            auto below = [](long long n) { return n <= 0 ? 0u : n >= kPage ? 0xffffu : (1u << (int)n) - 1u; };
+            auto seen = [&](int pg) {
+                const long long p0 = m.p0[pg];
+                uint32_t bits = below(pos + 1 - p0);
+                if (a.window) bits &= ~below(pos + 1ll - a.window - p0) | below(a.sinks - p0);
+                return bits;
+            };
+            // the step's largest score.  Loops stay rolled: what does not fit the instruction cache waits for it.
             float mx = -INFINITY;
+            if (!edge) {
+#pragma unroll 1
+                for (int ch = 0; ch < 4; ++ch) {
+                    int x[32];
+                    tmem_ld32(S + 32 * ch, x);
 #pragma unroll
-            for (int ch = 0; ch < 4; ++ch) {
-                int x[32];
-                tmem_ld32(S + 32 * ch, x);
+                    for (int e = 0; e < 2; ++e) {
+                        float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float ks = m.ks[2 * ch + e] * smul;
-                    float top = -INFINITY;
-                    if (edge) {
-                        const int p0 = m.p0[2 * ch + e];
-#pragma unroll
-                        for (int i = 0; i < kPage; ++i)
-                            top = fmaxf(top, hidden(p0 + i) ? -INFINITY : __int_as_float(x[16 * e + i]) * ks);
-                        mx = fmaxf(mx, top);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < kPage; ++i) top = fmaxf(top, __int_as_float(x[16 * e + i]));
-                        mx = fmaxf(mx, top * ks);
+                        for (int i = 0; i < kPage; i += 4) {
+                            t0 = fmaxf(fmaxf(t0, __int_as_float(x[16 * e + i])), __int_as_float(x[16 * e + i + 1]));
+                            t1 = fmaxf(fmaxf(t1, __int_as_float(x[16 * e + i + 2])), __int_as_float(x[16 * e + i + 3]));
+                        }
+                        mx = fmaxf(mx, fmaxf(t0, t1) * (m.ks[2 * ch + e] * smul));
                     }
+                }
+            } else {
+                vmax = 0.f;
+#pragma unroll 1
+                for (int pg = 0; pg < kPPages; ++pg) {
+                    int x[16];
+                    tmem_ld16(S + 16 * pg, x);
+                    const uint32_t bits = seen(pg);
+                    const float ks = m.ks[pg] * smul;
+                    if (bits) vmax = fmaxf(vmax, m.vs[pg]);
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < kPage; ++i) top = fmaxf(top, bits >> i & 1 ? __int_as_float(x[i]) : -INFINITY);
+                    if (top > -INFINITY) mx = fmaxf(mx, top * ks);
                 }
             }
-            const bool far = mx > ref + kPSlack;  // true for the first finite one
-            if (__any_sync(kAll, far || vmax > vref)) {
-                const float r2 = far ? mx : ref;
-                // a power of two from vmax on
-                const float v2 = vmax > vref ? __uint_as_float((__float_as_uint(vmax) + 0x7fffffu) & 0x7f800000u) : vref;
-                const float fl = ref == r2 ? 1.f : ex2(ref - r2), f = fl * (vref / v2);
-                l *= fl;
-                if (done) {
+            // a power of two from vmax on
+            const float v2 = __uint_as_float((__float_as_uint(vmax) + 0x7fffffu) & 0x7f800000u);
+            if (wide) {
+                ref = mx;
+                vref = fmaxf(v2, 7.8886090522101181e-31f);
+            } else {
+                const bool far = mx > ref + kPSlack;  // true for the first finite one
+                if (__any_sync(kAll, far || vmax > vref)) {
+                    const float r2 = far ? mx : ref, vn = vmax > vref ? v2 : vref;
+                    const float fl = ref == r2 ? 1.f : ex2(ref - r2), f = fl * (vref / vn);
+                    l *= fl;
+                    if (done) {
+#pragma unroll 2
+                        for (int ch = 0; ch < HD / 16; ++ch) {
+                            int x[16];
+                            uint32_t y[16];
+                            tmem_ld16(O + 16 * ch, x);
 #pragma unroll
-                    for (int ch = 0; ch < HD / 16; ++ch) {
-                        int x[16];
-                        uint32_t y[16];
-                        tmem_ld16(O + 16 * ch, x);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__int_as_float(x[i]) * f);
-                        tmem_st16(O + 16 * ch, y);
+                            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__int_as_float(x[i]) * f);
+                            tmem_st16(O + 16 * ch, y);
+                        }
                     }
+                    ref = r2;
+                    vref = vn;
                 }
-                ref = r2;
-                vref = v2;
             }
             const float base = ref == -INFINITY ? 0.f : ref;
-            const float vmul = kPTop / vref;
+            const float vmul = (wide ? kPStepTop : kPTop) / vref;
             float l0 = 0.f, l1 = 0.f;
+            auto weights = [&](auto masked) {
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int ch = 0; ch < 4; ++ch) {
-                int x[32];
-                uint32_t hi16[16], lo16[16];
-                tmem_ld32(S + 32 * ch, x);
+                    for (int c2 = 0; c2 < 2; ++c2) {
+                        const int ch = 2 * h + c2;
+                        int x[32];
+                        uint32_t hi16[16], lo16[16];
+                        tmem_ld32(S + 32 * ch, x);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float ks = m.ks[2 * ch + e] * smul, vs = m.vs[2 * ch + e] * vmul;
-                    const int p0 = m.p0[2 * ch + e];
+                        for (int e = 0; e < 2; ++e) {
+                            const float ks = m.ks[2 * ch + e] * smul, vs = m.vs[2 * ch + e] * vmul;
+                            const uint32_t bits = masked ? seen(2 * ch + e) : 0;
 #pragma unroll
-                    for (int i = 0; i < kPage; i += 2) {
-                        float p = ex2(fmaf(__int_as_float(x[16 * e + i]), ks, -base));
-                        float u = ex2(fmaf(__int_as_float(x[16 * e + i + 1]), ks, -base));
-                        float pv = p * vs, uv = u * vs;
-                        if (edge) {  // a hidden block's scales may be NaN
-                            if (hidden(p0 + i)) p = pv = 0.f;
-                            if (hidden(p0 + i + 1)) u = uv = 0.f;
+                            for (int i = 0; i < kPage; i += 2) {
+                                float p[2] = {-base, -base};
+                                fma2(p, ks, __int_as_float(x[16 * e + i]), __int_as_float(x[16 * e + i + 1]));
+                                p[0] = ex2(p[0]);
+                                p[1] = ex2(p[1]);
+                                if (masked) {  // a hidden block's scales may be NaN
+                                    p[0] = bits >> i & 1 ? p[0] : 0.f;
+                                    p[1] = bits >> (i + 1) & 1 ? p[1] : 0.f;
+                                }
+                                l0 += p[0];
+                                l1 += p[1];
+                                mul2(p, vs);
+                                if (masked) {
+                                    p[0] = bits >> i & 1 ? p[0] : 0.f;
+                                    p[1] = bits >> (i + 1) & 1 ? p[1] : 0.f;
+                                }
+                                hi16[8 * e + i / 2] = half2_bits(p[0], p[1]);
+                                if (wide) lo16[8 * e + i / 2] = left_over(p[0], p[1], hi16[8 * e + i / 2]);
+                            }
                         }
-                        l0 += p;
-                        l1 += u;
-                        hi16[8 * e + i / 2] = half2_bits(pv, uv);
-                        if (wide) lo16[8 * e + i / 2] = left_over(pv, uv, hi16[8 * e + i / 2]);
+                        tmem_st16(S + 32 * ch, hi16);
+                        if (wide) tmem_st16(S + 32 * ch + 16, lo16);
                     }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(&sm.pfull[w][h]);  // half of the keys' products may start
                 }
-                tmem_st16(S + 32 * ch, hi16);
-                if (wide) tmem_st16(S + 32 * ch + 16, lo16);
+            };
+            if (edge) weights(std::true_type());
+            else weights(std::false_type());
+            if (wide) {
+                sm.stat[t % kPMeta][row] = make_float4(ref, l0 + l1, vref * (1.f / kPStepTop), 0.f);
+                mbar_arrive(&sm.tfull[t % kPMeta]);
+                if (g > 0) ok = take(g - 1);
+            } else {
+                l += l0 + l1;
             }
-            l += l0 + l1;
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(&sm.pfull[w]);
+            ++done;
         }
-        if (ok && done) ok = mbar_wait(&sm.odone[w], 0, r.err, ERR_WAIT_FULL);
-        if (ok && split && w) ok = mbar_wait(&sm.odone[0], 0, r.err, ERR_WAIT_FULL);  // it stores where V was
-        ok = __all_sync(kAll, ok);
-        if (!ok) l = NAN;  // a wait ran out: the result says so
-        tc_fence_after();
-        float f = done ? vref * (1.f / kPTop) : 0.f;  // takes O to sums of weight * value
-        float *xch = reinterpret_cast<float *>(sm.k);  // [kPM][HD + 4], over K and V
-        if (split) {
-            if (w == 1) {
+        T *y = reinterpret_cast<T *>(a.out.p) + (long long)(row0 + ti) * a.out.row_stride +
+               (long long)(kvh * G + st - ti * G) * a.out.head_stride;
+        if (wide) {
+            if (ok) ok = take(jobs - 1);
+            if (!__all_sync(kAll, ok)) sum = NAN;  // a wait ran out: the result says so
+            const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+            if (ls < nslots) {
 #pragma unroll
+                for (int i = 0; i < HALF; i += 4) {
+                    float z[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) z[e] = acc[(i + e) % HALF] * inv;
+                    store_n<4>(y + w * HALF + i, vec, z);
+                }
+            }
+        } else {
+            if (ok && done) ok = mbar_wait(&sm.odone[w], 0, r.err, ERR_WAIT_FULL);
+            if (ok && split && w) ok = mbar_wait(&sm.odone[0], 0, r.err, ERR_WAIT_FULL);  // it stores where V was
+            ok = __all_sync(kAll, ok);
+            if (!ok) l = NAN;
+            tc_fence_after();
+            float f = done ? vref * (1.f / kPTop) : 0.f;   // takes O to sums of weight * value
+            float *xch = reinterpret_cast<float *>(sm.k);  // [kPM][HD + 4], over K and V
+            if (split) {
+                if (w == 1) {
+#pragma unroll 1
+                    for (int ch = 0; ch < HD / 16; ++ch) {
+                        int x[16];
+                        if (done) tmem_ld16(O + 16 * ch, x);
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4)
+                            *reinterpret_cast<float4 *>(&xch[row * (HD + 4) + 16 * ch + i]) =
+                                done ? make_float4(__int_as_float(x[i]) * f, __int_as_float(x[i + 1]) * f,
+                                                   __int_as_float(x[i + 2]) * f, __int_as_float(x[i + 3]) * f)
+                                     : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+                    sm.join[0][row] = ref;
+                    sm.join[1][row] = l;
+                }
+                named_sync(1, 2 * kPM);
+            }
+            if ((!split || w == 0) && ls - lane < nslots) {
+                float g1 = 0.f;
+                if (split) {
+                    const float ref1 = sm.join[0][row], top = fmaxf(ref, ref1);
+                    const float g0 = ref == -INFINITY ? 0.f : ex2(ref - top);
+                    g1 = ref1 == -INFINITY ? 0.f : ex2(ref1 - top);
+                    l = g0 * l + g1 * sm.join[1][row];
+                    f *= g0;
+                }
+                const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+#pragma unroll 1
                 for (int ch = 0; ch < HD / 16; ++ch) {
                     int x[16];
-                    if (done) tmem_ld16(O + 16 * ch, x);
+                    tmem_ld16(O + 16 * ch, x);
+                    if (ls < nslots) {
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4)
-                        *reinterpret_cast<float4 *>(&xch[row * (HD + 4) + 16 * ch + i]) =
-                            done ? make_float4(__int_as_float(x[i]) * f, __int_as_float(x[i + 1]) * f,
-                                               __int_as_float(x[i + 2]) * f, __int_as_float(x[i + 3]) * f)
-                                 : make_float4(0.f, 0.f, 0.f, 0.f);
-                }
-                sm.join[0][row] = ref;
-                sm.join[1][row] = l;
-            }
-            named_sync(1, 2 * kPM);
-        }
-        if ((!split || w == 0) && ls - lane < nslots) {
-            float g1 = 0.f;
-            if (split) {
-                const float ref1 = sm.join[0][row], top = fmaxf(ref, ref1);
-                const float g0 = ref == -INFINITY ? 0.f : ex2(ref - top);
-                g1 = ref1 == -INFINITY ? 0.f : ex2(ref1 - top);
-                l = g0 * l + g1 * sm.join[1][row];
-                f *= g0;
-            }
-            const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
-            T *y = reinterpret_cast<T *>(a.out.p) + (long long)(row0 + ti) * a.out.row_stride +
-                   (long long)(kvh * G + st - ti * G) * a.out.head_stride;
+                        for (int i = 0; i < 16; i += 4) {
+                            float z[4];
 #pragma unroll
-            for (int ch = 0; ch < HD / 16; ++ch) {
-                int x[16];
-                tmem_ld16(O + 16 * ch, x);
-                if (ls < nslots) {
+                            for (int e = 0; e < 4; ++e) z[e] = __int_as_float(x[i + e]) * f;
+                            if (split) {
+                                const float4 o1 = *reinterpret_cast<const float4 *>(&xch[row * (HD + 4) + 16 * ch + i]);
+                                z[0] += g1 * o1.x, z[1] += g1 * o1.y, z[2] += g1 * o1.z, z[3] += g1 * o1.w;
+                            }
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        float z[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) z[e] = __int_as_float(x[i + e]) * f;
-                        if (split) {
-                            const float4 o1 = *reinterpret_cast<const float4 *>(&xch[row * (HD + 4) + 16 * ch + i]);
-                            z[0] += g1 * o1.x, z[1] += g1 * o1.y, z[2] += g1 * o1.z, z[3] += g1 * o1.w;
+                            for (int e = 0; e < 4; ++e) z[e] *= inv;
+                            store_n<4>(y + 16 * ch + i, vec, z);
                         }
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) z[e] *= inv;
-                        store_n<4>(y + 16 * ch + i, vec, z);
                     }
                 }
             }
