@@ -8,13 +8,13 @@
 // and SM takes as long as the products at head_dim 128 and twice as long at 64.
 //
 // One CTA per tile of slots; a step is 128 keys (8 pages):
-//   warps 8-11   producers: int8 pages -> f16 operands in shared memory, two
+//   warps 0-3    producers: int8 pages -> f16 operands in shared memory, two
 //                steps deep (128-byte swizzled rows, K-major: keys [key][dim],
 //                values [dim][key], which is how the cache holds them).  Every
 //                int8 is exact in f16; the blocks' scales stay apart.
-//   warp 12      one lane issues the products: S = Q K^T (128 x 128, f32 in
+//   warp 4       one lane issues the products: S = Q K^T (128 x 128, f32 in
 //                TMEM), O += P V with P from TMEM.
-//   warps 0-3, 4-7   two groups of one row per thread: softmax of S, P as f16
+//   warps 8-11, 12-15   two groups of one row per thread: softmax of S, P as f16
 //                over S's own columns, the output.
 // The groups take turns: while one forms its weights, the other's products
 // run.  f16 / bf16 rows: 256 slots, 128 per group, every step.  A last tile of
@@ -44,7 +44,7 @@ namespace s2k {
 
 constexpr int kPM = 128;        // slots of a group, keys of a step
 constexpr int kPPages = kPM / kPage;
-constexpr int kPThreads = 512;  // warps 13-15 only make the register shares whole groups of four warps
+constexpr int kPThreads = 512;  // warps 5-7 only make the register shares whole groups of four warps
 constexpr int kPMeta = 4;       // steps whose scales and positions are held
 constexpr float kPTop = 128.f;  // a weight at its reference, with the largest value scale
 constexpr float kPStepTop = 16384.f;  // the same for f32 rows, whose reference is the step's maximum
@@ -165,17 +165,17 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
         }
         fence_mbar_init();
     }
-    if (warp == 12) {
+    if (warp == 4) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     // queries -> f16 operands, a warp a slot at a time
-    if (warp < 8) {
+    if (warp >= 8) {
         constexpr int E = HD / 32;
         const float sign = a.scale < 0.f ? -1.f : 1.f;
         const int half = nslots > kPM ? 2 * kPM : kPM;
-        for (int s = warp; s < half; s += 8) {
+        for (int s = warp - 8; s < half; s += 8) {
             const int st = slot0 + min(s, nslots - 1), row = st / G;
             float x[E];
             load_n<E>(reinterpret_cast<const T *>(a.q.p) + (long long)(row0 + row) * a.q.row_stride +
@@ -213,27 +213,37 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
     bool ok = true;
 
     // registers: 512 threads start with 128 each, and 2 * 168 + 96 + 72 <= 4 * 128
-    if (warp >= 8 && warp < 12) {
+    if (warp < 4) {
         // ---------------- producers: two pages of each step per warp ----------------
         asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-        const int pw = warp - 8;
+        const int pw = warp;
         constexpr int U = HD / 32;  // 16-byte pieces per lane and page
         uint4 kr[2][U], vr[2][U];
-        auto pages_of = [&](int t, int (&pg)[2]) {  // lanes 0 and 1 look them up
+        // lanes 0 and 1 look up the warp's two pages, a step before anything depends on them
+        auto first_token = [&](int t) {
             const int x = t * kPPages + 2 * pw + (lane & 1);
-            const int lg = x < ns ? x : x - ns + fw;
-            const int p = t < steps && x < total && lane < 2 ? kv8_page(c, r, b, lg) : -1;
-            pg[0] = __shfl_sync(kAll, p, 0);
-            pg[1] = __shfl_sync(kAll, p, 1);
+            return t < steps && x < total ? (x < ns ? x : x - ns + fw) * kPage : kPNone;
         };
+        auto look_up = [&](int t) {
+            const int p0 = first_token(t);
+            return lane < 2 && p0 != kPNone ? kv8_page(c, r, b, p0 / kPage) : -1;
+        };
+        auto scales = [&](int page, float &ks, float &vs) {
+            ks = vs = 0.f;
+            if (page >= 0) {
+                ks = c.k_scale[c.block(page, kvh)];
+                vs = c.v_scale[c.block(page, kvh)];
+            }
+        };
+        // where there is no page, page 0's: its tokens are behind every position, so nothing of them is used
+        // (loads under a condition were waited for one by one, 4400 cycles a step)
         auto fetch = [&](const int8_t *src, const int (&pg)[2], uint4 (&x)[2][U]) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 2; ++e) {
+                const uint4 *p = reinterpret_cast<const uint4 *>(src + c.block(max(pg[e], 0), kvh) * (kPage * HD)) + lane;
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-                    x[e][u] = pg[e] >= 0 ? *reinterpret_cast<const uint4 *>(src + c.block(pg[e], kvh) * (kPage * HD) +
-                                                                          (u * 32 + lane) * 16)
-                                         : make_uint4(0, 0, 0, 0);
+                for (int u = 0; u < U; ++u) x[e][u] = __ldg(p + u * 32);
+            }
         };
         auto put = [&](uint8_t *buf, int row, int piece, uint32_t w0, uint32_t w1) {
             uint4 h;
@@ -241,21 +251,23 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             cvt_i8x4(w1, h.z, h.w);
             *reinterpret_cast<uint4 *>(buf + swz(row, piece)) = h;
         };
-        int pg[2], pn[2];
-        pages_of(0, pg);
+        int pg[2], own = look_up(0), next = look_up(1), later;
+        float ks, vs;
+        pg[0] = __shfl_sync(kAll, own, 0);
+        pg[1] = __shfl_sync(kAll, own, 1);
         fetch(c.k, pg, kr);
+        scales(own, ks, vs);
         for (int t = 0; t < steps && ok; ++t) {
             const int s = t & 1;
             fetch(c.v, pg, vr);
-            pages_of(t + 1, pn);
+            later = look_up(t + 2);
             if (t >= 2) ok = mbar_wait(&sm.kempty[s], ((t >> 1) - 1) & 1, r.err, ERR_WAIT_EMPTY);
             if (!(ok = __all_sync(kAll, ok))) break;
             if (lane < 2) {
                 typename Sm::Meta &m = sm.meta[t % kPMeta];
-                const int i = 2 * pw + lane, p = lane ? pg[1] : pg[0], x = t * kPPages + i;
-                m.ks[i] = p >= 0 ? c.k_scale[c.block(p, kvh)] : 0.f;
-                m.vs[i] = p >= 0 ? c.v_scale[c.block(p, kvh)] : 0.f;
-                m.p0[i] = p >= 0 ? (x < ns ? x : x - ns + fw) * kPage : kPNone;
+                m.ks[2 * pw + lane] = ks;
+                m.vs[2 * pw + lane] = vs;
+                m.p0[2 * pw + lane] = own >= 0 ? first_token(t) : kPNone;
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.mfull[t % kPMeta]);
@@ -275,7 +287,12 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.kfull[s]);
-            fetch(c.k, pn, kr);
+            own = next;
+            next = later;
+            pg[0] = __shfl_sync(kAll, own, 0);
+            pg[1] = __shfl_sync(kAll, own, 1);
+            fetch(c.k, pg, kr);
+            scales(own, ks, vs);
             if (t >= 2) ok = mbar_wait(&sm.vempty[s], ((t >> 1) - 1) & 1, r.err, ERR_WAIT_EMPTY);
             if (!(ok = __all_sync(kAll, ok))) break;
 #pragma unroll
@@ -291,12 +308,11 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.vfull[s]);
-            pg[0] = pn[0], pg[1] = pn[1];
         }
-    } else if (warp >= 12) {
+    } else if (warp < 8) {
         // ---------------- products ----------------
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == 12 && lane == 0) {
+        if (warp == 4 && lane == 0) {
             // an operand's next 16 columns of K are 32 bytes on, the next 64 a chunk
             const uint64_t q0 = sw128_desc(sm.q[0][0]), q1 = sw128_desc(sm.q[1][0]);
             auto at = [](int x, int chunk) { return (uint64_t)(2 * (x % 4) + (x / 4) * (chunk >> 4)); };
@@ -345,7 +361,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
     } else {
         // ---------------- softmax: one row per thread ----------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
-        const int w = warp >> 2, row = tid & (kPM - 1), ls = (split ? 0 : w * kPM) + row;
+        const int w = (warp >> 2) - 2, row = tid & (kPM - 1), ls = (split ? 0 : w * kPM) + row;
         const int st = slot0 + min(ls, nslots - 1), ti = st / G;
         const int pos = past + ti;
         // positions of the warp's rows
@@ -605,7 +621,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 4) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
