@@ -66,7 +66,7 @@ struct PromptSmem {
     float join[2][kPM];
     float4 stat[kPMeta][kPM];  // f32 rows: a step's reference, sum and what an O of 1 is worth
     uint64_t kfull[2], kempty[2], vfull[2], vempty[2], mfull[kPMeta], sfull[2], pfull[2][2], odone[2];
-    uint64_t tfull[kPMeta], ofree[2];
+    uint64_t tfull[kPMeta], ofree[2], qfull;
     uint32_t tmem;
 };
 
@@ -123,7 +123,7 @@ __device__ __forceinline__ uint32_t left_over(float x, float y, uint32_t h) {
 __device__ __forceinline__ int swz(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
 
 template <int HD, int TYPE>
-__global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows r, Kv8Attn a, int vec) {
+__global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows r, Kv8Attn a, int vec_q, int vec_out) {
     using T = typename OType<TYPE>::T;
     using Sm = PromptSmem<HD>;
     constexpr bool wide = TYPE == OT_F32;
@@ -159,6 +159,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             mbar_init(&sm.odone[i], 1);
             mbar_init(&sm.ofree[i], 2 * kPM);
         }
+        mbar_init(&sm.qfull, 8);
         for (int i = 0; i < kPMeta; ++i) {
             mbar_init(&sm.mfull[i], 4);
             mbar_init(&sm.tfull[i], kPM);
@@ -169,42 +170,6 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    // queries -> f16 operands, a warp a slot at a time
-    if (warp >= 8) {
-        constexpr int E = HD / 32;
-        const float sign = a.scale < 0.f ? -1.f : 1.f;
-        const int half = nslots > kPM ? 2 * kPM : kPM;
-        for (int s = warp - 8; s < half; s += 8) {
-            const int st = slot0 + min(s, nslots - 1), row = st / G;
-            float x[E];
-            load_n<E>(reinterpret_cast<const T *>(a.q.p) + (long long)(row0 + row) * a.q.row_stride +
-                          (long long)(kvh * G + st - row * G) * a.q.head_stride + lane * E,
-                      vec, x);
-            unsigned top = 0;
-#pragma unroll
-            for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-            top = __reduce_max_sync(kAll, top);
-            // 2^-e brings the slot's largest to 2^13 .. 2^14
-            const int e2 = max((int)(top >> 23) - 127, -112) - 13;
-            const float down = sign * __int_as_float((127 - e2) << 23);
-            if (lane == 0)
-                sm.qmul[s / kPM][s % kPM] =
-                    top >= 0x7f800000u ? NAN : fabsf(a.scale) * 1.44269504f * __int_as_float((e2 + 127) << 23);
-            uint32_t h[E / 2], lo[E / 2];
-#pragma unroll
-            for (int e = 0; e < E / 2; ++e) {
-                h[e] = half2_bits(x[2 * e] * down, x[2 * e + 1] * down);
-                lo[e] = wide ? left_over(x[2 * e] * down, x[2 * e + 1] * down, h[e]) : 0;
-            }
-            const int dim = lane * E, at = swz(s % kPM, dim % 64 / 8) + dim % 8 * 2;
-#pragma unroll
-            for (int e = 0; e < E / 2; ++e) {
-                *reinterpret_cast<uint32_t *>(&sm.q[s / kPM][dim / 64][at + 4 * e]) = h[e];
-                if (wide) *reinterpret_cast<uint32_t *>(&sm.q[1][dim / 64][at + 4 * e]) = lo[e];
-            }
-        }
-        fence_proxy_async_smem();
     }
     tc_fence_before();
     __syncthreads();
@@ -332,7 +297,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 if (split || w) mma_commit(&sm.kempty[s]);
                 return true;
             };
-            ok = qk(0);
+            ok = mbar_wait(&sm.qfull, 0, r.err, ERR_WAIT_FULL) && qk(0);
             if (ok && jobs > 1) ok = qk(1);
             for (int g = 0; g < jobs && ok; ++g) {
                 const int t = split ? g : g >> 1, w = g & 1, s = t & 1;
@@ -361,6 +326,49 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
     } else {
         // ---------------- softmax: one row per thread ----------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        // queries -> f16 operands, a warp eight slots at a time
+        {
+            constexpr int E = HD / 32, B = 8;
+            const float sign = a.scale < 0.f ? -1.f : 1.f;
+            const int dim = lane * E;
+            for (int s0 = (warp - 8) * B; s0 < (nslots > kPM ? 2 * kPM : kPM); s0 += 8 * B) {
+                float x[B][E];
+#pragma unroll
+                for (int i = 0; i < B; ++i) {
+                    const int st = slot0 + min(s0 + i, nslots - 1), row = st / G;
+                    load_n<E>(reinterpret_cast<const T *>(a.q.p) + (long long)(row0 + row) * a.q.row_stride +
+                                  (long long)(kvh * G + st - row * G) * a.q.head_stride + dim,
+                              vec_q, x[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < B; ++i) {
+                    const int s = s0 + i;
+                    unsigned top = 0;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(x[i][e]) & 0x7fffffffu);
+                    top = __reduce_max_sync(kAll, top);
+                    // 2^-e brings the slot's largest to 2^13 .. 2^14
+                    const int e2 = max((int)(top >> 23) - 127, -112) - 13;
+                    const float down = sign * __int_as_float((127 - e2) << 23);
+                    if (lane == 0)
+                        sm.qmul[s / kPM][s % kPM] =
+                            top >= 0x7f800000u ? NAN : fabsf(a.scale) * 1.44269504f * __int_as_float((e2 + 127) << 23);
+                    const int at = swz(s % kPM, dim % 64 / 8) + dim % 8 * 2;
+#pragma unroll
+                    for (int e = 0; e < E / 2; ++e) {
+                        const uint32_t h = half2_bits(x[i][2 * e] * down, x[i][2 * e + 1] * down);
+                        *reinterpret_cast<uint32_t *>(&sm.q[s / kPM][dim / 64][at + 4 * e]) = h;
+                        if (wide)
+                            *reinterpret_cast<uint32_t *>(&sm.q[1][dim / 64][at + 4 * e]) =
+                                left_over(x[i][2 * e] * down, x[i][2 * e + 1] * down, h);
+                    }
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.qfull);
+            ok = mbar_wait(&sm.qfull, 0, r.err, ERR_WAIT_FULL);
+        }
         const int w = (warp >> 2) - 2, row = tid & (kPM - 1), ls = (split ? 0 : w * kPM) + row;
         const int st = slot0 + min(ls, nslots - 1), ti = st / G;
         const int pos = past + ti;
@@ -545,21 +553,51 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             }
             ++done;
         }
-        T *y = reinterpret_cast<T *>(a.out.p) + (long long)(row0 + ti) * a.out.row_stride +
-               (long long)(kvh * G + st - ti * G) * a.out.head_stride;
+        // The group's outputs go out by way of its half of Q's memory (the products are done with it), so that a warp
+        // stores whole rows: pieces of 16 bytes, a row's pieces exchanged by its number to meet all banks.
+        constexpr int E = 16 / sizeof(T), PIECES = (wide ? HD / 2 : HD) / E;
+        uint8_t *stage = sm.q[w][0];
+        auto piece_at = [&](int rr, int piece) { return stage + (rr * PIECES + (piece ^ (rr & 7))) * 16; };
+        auto lay = [&](int first, const float (&z)[16]) {  // 16 dims of the thread's row
+#pragma unroll
+            for (int p = 0; p < 16 / E; ++p) {
+                Vec<T, E> u;
+#pragma unroll
+                for (int e = 0; e < E; ++e) u.v[e] = from_f<T>(z[p * E + e]);
+                *reinterpret_cast<Vec<T, E> *>(piece_at(row, first / E + p)) = u;
+            }
+        };
+        auto store_rows = [&](int dim0) {  // the warp's 32 rows, dims from dim0 on
+            __syncwarp();
+            constexpr int RPI = 32 / PIECES;  // rows per access
+#pragma unroll 4
+            for (int rr = 0; rr < 32; rr += RPI) {
+                const int rl = row - lane + rr + lane / PIECES, sl = ls - lane + rr + lane / PIECES, p = lane % PIECES;
+                if (sl >= nslots) break;
+                const int s2 = slot0 + sl, t2 = s2 / G;
+                T *y = reinterpret_cast<T *>(a.out.p) + (long long)(row0 + t2) * a.out.row_stride +
+                       (long long)(kvh * G + s2 - t2 * G) * a.out.head_stride + dim0 + p * E;
+                const Vec<T, E> u = *reinterpret_cast<const Vec<T, E> *>(piece_at(rl, p));
+                if (vec_out) {
+                    *reinterpret_cast<Vec<T, E> *>(y) = u;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) y[e] = u.v[e];
+                }
+            }
+        };
         if (wide) {
             if (ok) ok = take(jobs - 1);
             if (!__all_sync(kAll, ok)) sum = NAN;  // a wait ran out: the result says so
             const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-            if (ls < nslots) {
 #pragma unroll
-                for (int i = 0; i < HALF; i += 4) {
-                    float z[4];
+            for (int i = 0; i < HALF; i += 16) {
+                float z[16];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) z[e] = acc[(i + e) % HALF] * inv;
-                    store_n<4>(y + w * HALF + i, vec, z);
-                }
+                for (int e = 0; e < 16; ++e) z[e] = acc[(i + e) % HALF] * inv;
+                lay(i, z);
             }
+            store_rows(w * HALF);
         } else {
             if (ok && done) ok = mbar_wait(&sm.odone[w], 0, r.err, ERR_WAIT_FULL);
             if (ok && split && w) ok = mbar_wait(&sm.odone[0], 0, r.err, ERR_WAIT_FULL);  // it stores where V was
@@ -600,22 +638,21 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 for (int ch = 0; ch < HD / 16; ++ch) {
                     int x[16];
                     tmem_ld16(O + 16 * ch, x);
-                    if (ls < nslots) {
+                    float z[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) z[i] = __int_as_float(x[i]) * f;
+                    if (split) {
 #pragma unroll
                         for (int i = 0; i < 16; i += 4) {
-                            float z[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) z[e] = __int_as_float(x[i + e]) * f;
-                            if (split) {
-                                const float4 o1 = *reinterpret_cast<const float4 *>(&xch[row * (HD + 4) + 16 * ch + i]);
-                                z[0] += g1 * o1.x, z[1] += g1 * o1.y, z[2] += g1 * o1.z, z[3] += g1 * o1.w;
-                            }
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) z[e] *= inv;
-                            store_n<4>(y + 16 * ch + i, vec, z);
+                            const float4 o1 = *reinterpret_cast<const float4 *>(&xch[row * (HD + 4) + 16 * ch + i]);
+                            z[i] += g1 * o1.x, z[i + 1] += g1 * o1.y, z[i + 2] += g1 * o1.z, z[i + 3] += g1 * o1.w;
                         }
                     }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) z[i] *= inv;
+                    lay(16 * ch, z);
                 }
+                store_rows(0);
             }
         }
     }
@@ -655,10 +692,10 @@ cudaError_t launch_kv8_prompt(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, 
     const long long tiles = (slots + per - 1) / per;
     if (slots > 0x7fffffffLL || tiles * r.n_seqs > 0x7fffffffLL) return cudaErrorInvalidValue;
     const dim3 grid((unsigned)(tiles * r.n_seqs), c.n_kv_heads);
-    const int vec = rows_vec(a.q, 4) && rows_vec(a.out, 4);
+    const int vec_q = rows_vec(a.q, c.head_dim / 32), vec_out = rows_vec(a.out, a.out.type == OT_F32 ? 4 : 8);
     count_launch();
     return kv8_dispatch(c.head_dim, a.q.type, [&](auto h, auto t) {
-        kv8_prompt_kernel<h, t><<<grid, kPThreads, prompt_smem<h>(), st>>>(c, r, a, vec);
+        kv8_prompt_kernel<h, t><<<grid, kPThreads, prompt_smem<h>(), st>>>(c, r, a, vec_q, vec_out);
         return cudaGetLastError();
     });
 }
