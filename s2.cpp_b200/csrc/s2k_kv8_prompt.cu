@@ -75,18 +75,23 @@ template <int N>
 constexpr uint32_t prompt_idesc() {
     return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kPM >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int acc) {
+// An operand's descriptor (sw128_desc) by its low word: the high word is the
+// same for all, and 64-bit sums per product kept the issuing lane behind the
+// tensor cores.
+constexpr uint32_t kDescHigh = (uint32_t)((1024 >> 4) | (1u << 14) | (2u << 29));
+__device__ __forceinline__ uint32_t desc_low(const void *p) { return ((smem_u32(p) >> 4) & 0x3fff) | 1u << 16; }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\t"
+        "mov.b64 b, {%2, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kDescHigh)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, int acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kDescHigh)
         : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
@@ -137,9 +142,13 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
     const int G = a.n_heads / c.n_kv_heads;
     int row0, n, past;
     if (!kv8_seq(r, b, row0, n, past) || (long long)tile * SLOTS >= (long long)n * G) return;
+    // a slot's row: exact in f32 below 2^20 slots
+    const bool few = (long long)n * G < 1 << 20;
+    const float inv_group = 1.f / (float)G;
+    auto row_of = [&](int slot) { return few ? (int)(((float)slot + 0.5f) * inv_group) : slot / G; };
     const int slot0 = tile * SLOTS, nslots = (int)min((long long)SLOTS, (long long)n * G - slot0);
     const bool split = wide || nslots <= kPM;  // the groups share the slots and alternate in steps
-    const int pos_lo = past + slot0 / G, pos_hi = past + (slot0 + nslots - 1) / G;
+    const int pos_lo = past + row_of(slot0), pos_hi = past + row_of(slot0 + nslots - 1);
     const int wlo = a.window ? max(pos_lo - a.window + 1, 0) : 0;
     const int fw = wlo / kPage;
     const int ns = min((int)(((long long)a.sinks + kPage - 1) / kPage), fw);
@@ -279,18 +288,18 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 4 && lane == 0) {
             // an operand's next 16 columns of K are 32 bytes on, the next 64 a chunk
-            const uint64_t q0 = sw128_desc(sm.q[0][0]), q1 = sw128_desc(sm.q[1][0]);
-            auto at = [](int x, int chunk) { return (uint64_t)(2 * (x % 4) + (x / 4) * (chunk >> 4)); };
+            const uint32_t q0 = desc_low(sm.q[0][0]), q1 = desc_low(sm.q[1][0]);
+            auto at = [](int x, int chunk) { return (uint32_t)(2 * (x % 4) + (x / 4) * (chunk >> 4)); };
             auto qk = [&](int g) {
                 const int t = split ? g : g >> 1, w = g & 1, s = t & 1;
                 if (!mbar_wait(&sm.kfull[s], (t >> 1) & 1, r.err, ERR_WAIT_FULL)) return false;
                 tc_fence_after();
                 const uint32_t d = tmem + w * kPM;
-                const uint64_t q = !split && w ? q1 : q0, k = sw128_desc(sm.k[s][0]);
-#pragma unroll 2
+                const uint32_t q = !split && w ? q1 : q0, k = desc_low(sm.k[s][0]);
+#pragma unroll
                 for (int x = 0; x < 4 * NC; ++x) mma_ss(d, q + at(x, kPM * 128), k + at(x, kPM * 128), prompt_idesc<kPM>(), x != 0);
                 if (wide) {
-#pragma unroll 2
+#pragma unroll
                     for (int x = 0; x < 4 * NC; ++x) mma_ss(d, q1 + at(x, kPM * 128), k + at(x, kPM * 128), prompt_idesc<kPM>(), 1);
                 }
                 mma_commit(&sm.sfull[w]);
@@ -302,16 +311,16 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             for (int g = 0; g < jobs && ok; ++g) {
                 const int t = split ? g : g >> 1, w = g & 1, s = t & 1;
                 const uint32_t d = tmem + 2 * kPM + w * kPM, p = tmem + w * kPM;
-                const uint64_t v = sw128_desc(sm.v[s][0]);
+                const uint32_t v = desc_low(sm.v[s][0]);
                 ok = mbar_wait(&sm.vfull[s], (t >> 1) & 1, r.err, ERR_WAIT_FULL);
                 // f32 rows: the output of two steps ago has been taken
                 if (ok && wide && g > 1) ok = mbar_wait(&sm.ofree[w], ((g >> 1) - 1) & 1, r.err, ERR_WAIT_EMPTY);
                 for (int h = 0; h < 2 && ok; ++h) {  // 64 keys each
                     if (!(ok = mbar_wait(&sm.pfull[w][h], (g >> 1) & 1, r.err, ERR_WAIT_FULL))) break;
                     tc_fence_after();
-#pragma unroll 2
+#pragma unroll
                     for (int y = 0; y < 4; ++y) {
-                        const uint64_t vx = v + at(y, 0) + h * (HD * 128 >> 4);
+                        const uint32_t vx = v + at(y, 0) + h * (HD * 128 >> 4);
                         const uint32_t px = p + 64 * h + 32 * (y / 2) + 8 * (y % 2);
                         mma_ts(d, px, vx, prompt_idesc<HD>(), (!wide && g > 1) || h > 0 || y > 0);
                         if (wide) mma_ts(d, px + 16, vx, prompt_idesc<HD>(), 1);
@@ -335,7 +344,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 float x[B][E];
 #pragma unroll
                 for (int i = 0; i < B; ++i) {
-                    const int st = slot0 + min(s0 + i, nslots - 1), row = st / G;
+                    const int st = slot0 + min(s0 + i, nslots - 1), row = row_of(st);
                     load_n<E>(reinterpret_cast<const T *>(a.q.p) + (long long)(row0 + row) * a.q.row_stride +
                                   (long long)(kvh * G + st - row * G) * a.q.head_stride + dim,
                               vec_q, x[i]);
@@ -370,11 +379,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             ok = mbar_wait(&sm.qfull, 0, r.err, ERR_WAIT_FULL);
         }
         const int w = (warp >> 2) - 2, row = tid & (kPM - 1), ls = (split ? 0 : w * kPM) + row;
-        const int st = slot0 + min(ls, nslots - 1), ti = st / G;
-        const int pos = past + ti;
+        const int pos = past + row_of(slot0 + min(ls, nslots - 1));
         // positions of the warp's rows
         const int s_lo = slot0 + min(ls - lane, nslots - 1), s_hi = slot0 + min(ls - lane + 31, nslots - 1);
-        const int p_min = past + s_lo / G, p_max = past + s_hi / G;
+        const int p_min = past + row_of(s_lo), p_max = past + row_of(s_hi);
         const float smul = sm.qmul[split ? 0 : w][row];
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t S = tmem + lanes + w * kPM, O = tmem + lanes + 2 * kPM + w * kPM;
@@ -438,20 +446,21 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 if (a.window) bits &= ~below(pos + 1ll - a.window - p0) | below(a.sinks - p0);
                 return bits;
             };
-            // the step's largest score.  Loops stay rolled: what does not fit the instruction cache waits for it.
+            // the step's largest score.  Loops stay rolled: unrolled, with the next columns' loads ahead, they took twice
+            // as long (the instruction cache serves ten warps in five places).
             float mx = -INFINITY;
             if (!edge) {
 #pragma unroll 1
                 for (int ch = 0; ch < 4; ++ch) {
-                    int x[32];
-                    tmem_ld32(S + 32 * ch, x);
+                    int y[32];
+                    tmem_ld32(S + 32 * ch, y);
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
                         for (int i = 0; i < kPage; i += 4) {
-                            t0 = fmaxf(fmaxf(t0, __int_as_float(x[16 * e + i])), __int_as_float(x[16 * e + i + 1]));
-                            t1 = fmaxf(fmaxf(t1, __int_as_float(x[16 * e + i + 2])), __int_as_float(x[16 * e + i + 3]));
+                            t0 = fmaxf(fmaxf(t0, __int_as_float(y[16 * e + i])), __int_as_float(y[16 * e + i + 1]));
+                            t1 = fmaxf(fmaxf(t1, __int_as_float(y[16 * e + i + 2])), __int_as_float(y[16 * e + i + 3]));
                         }
                         mx = fmaxf(mx, fmaxf(t0, t1) * (m.ks[2 * ch + e] * smul));
                     }
@@ -460,14 +469,14 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 vmax = 0.f;
 #pragma unroll 1
                 for (int pg = 0; pg < kPPages; ++pg) {
-                    int x[16];
-                    tmem_ld16(S + 16 * pg, x);
+                    int y[16];
+                    tmem_ld16(S + 16 * pg, y);
                     const uint32_t bits = seen(pg);
                     const float ks = m.ks[pg] * smul;
                     if (bits) vmax = fmaxf(vmax, m.vs[pg]);
                     float top = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < kPage; ++i) top = fmaxf(top, bits >> i & 1 ? __int_as_float(x[i]) : -INFINITY);
+                    for (int i = 0; i < kPage; ++i) top = fmaxf(top, bits >> i & 1 ? __int_as_float(y[i]) : -INFINITY);
                     if (top > -INFINITY) mx = fmaxf(mx, top * ks);
                 }
             }
@@ -485,11 +494,11 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                     if (done) {
 #pragma unroll 2
                         for (int ch = 0; ch < HD / 16; ++ch) {
-                            int x[16];
+                            int z[16];
                             uint32_t y[16];
-                            tmem_ld16(O + 16 * ch, x);
+                            tmem_ld16(O + 16 * ch, z);
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__int_as_float(x[i]) * f);
+                            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__int_as_float(z[i]) * f);
                             tmem_st16(O + 16 * ch, y);
                         }
                     }
@@ -500,50 +509,52 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             const float base = ref == -INFINITY ? 0.f : ref;
             const float vmul = (wide ? kPStepTop : kPTop) / vref;
             float l0 = 0.f, l1 = 0.f;
-            auto weights = [&](auto masked) {
-#pragma unroll 1
-                for (int h = 0; h < 2; ++h) {
+            auto weights = [&](int ch, const int(&y)[32], auto masked) {
+                uint32_t hi16[16], lo16[16];
 #pragma unroll
-                    for (int c2 = 0; c2 < 2; ++c2) {
-                        const int ch = 2 * h + c2;
-                        int x[32];
-                        uint32_t hi16[16], lo16[16];
-                        tmem_ld32(S + 32 * ch, x);
+                for (int e = 0; e < 2; ++e) {
+                    const float ks = m.ks[2 * ch + e] * smul, vs = m.vs[2 * ch + e] * vmul;
+                    const uint32_t bits = masked ? seen(2 * ch + e) : 0;
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float ks = m.ks[2 * ch + e] * smul, vs = m.vs[2 * ch + e] * vmul;
-                            const uint32_t bits = masked ? seen(2 * ch + e) : 0;
-#pragma unroll
-                            for (int i = 0; i < kPage; i += 2) {
-                                float p[2] = {-base, -base};
-                                fma2(p, ks, __int_as_float(x[16 * e + i]), __int_as_float(x[16 * e + i + 1]));
-                                p[0] = ex2(p[0]);
-                                p[1] = ex2(p[1]);
-                                if (masked) {  // a hidden block's scales may be NaN
-                                    p[0] = bits >> i & 1 ? p[0] : 0.f;
-                                    p[1] = bits >> (i + 1) & 1 ? p[1] : 0.f;
-                                }
-                                l0 += p[0];
-                                l1 += p[1];
-                                mul2(p, vs);
-                                if (masked) {
-                                    p[0] = bits >> i & 1 ? p[0] : 0.f;
-                                    p[1] = bits >> (i + 1) & 1 ? p[1] : 0.f;
-                                }
-                                hi16[8 * e + i / 2] = half2_bits(p[0], p[1]);
-                                if (wide) lo16[8 * e + i / 2] = left_over(p[0], p[1], hi16[8 * e + i / 2]);
-                            }
+                    for (int i = 0; i < kPage; i += 2) {
+                        float p[2] = {-base, -base};
+                        fma2(p, ks, __int_as_float(y[16 * e + i]), __int_as_float(y[16 * e + i + 1]));
+                        p[0] = ex2(p[0]);
+                        p[1] = ex2(p[1]);
+                        if (masked) {  // a hidden block's scales may be NaN
+                            p[0] = bits >> i & 1 ? p[0] : 0.f;
+                            p[1] = bits >> (i + 1) & 1 ? p[1] : 0.f;
                         }
-                        tmem_st16(S + 32 * ch, hi16);
-                        if (wide) tmem_st16(S + 32 * ch + 16, lo16);
+                        l0 += p[0];
+                        l1 += p[1];
+                        mul2(p, vs);
+                        if (masked) {
+                            p[0] = bits >> i & 1 ? p[0] : 0.f;
+                            p[1] = bits >> (i + 1) & 1 ? p[1] : 0.f;
+                        }
+                        hi16[8 * e + i / 2] = half2_bits(p[0], p[1]);
+                        if (wide) lo16[8 * e + i / 2] = left_over(p[0], p[1], hi16[8 * e + i / 2]);
                     }
-                    tmem_wait_st();
-                    tc_fence_before();
-                    mbar_arrive(&sm.pfull[w][h]);  // half of the keys' products may start
+                }
+                tmem_st16(S + 32 * ch, hi16);
+                if (wide) tmem_st16(S + 32 * ch + 16, lo16);
+            };
+            auto half_done = [&](int h) {  // its products may start
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(&sm.pfull[w][h]);
+            };
+            auto all_weights = [&](auto masked) {
+#pragma unroll 1
+                for (int ch = 0; ch < 4; ++ch) {
+                    int y[32];
+                    tmem_ld32(S + 32 * ch, y);
+                    weights(ch, y, masked);
+                    if (ch & 1) half_done(ch / 2);
                 }
             };
-            if (edge) weights(std::true_type());
-            else weights(std::false_type());
+            if (edge) all_weights(std::true_type());
+            else all_weights(std::false_type());
             if (wide) {
                 sm.stat[t % kPMeta][row] = make_float4(ref, l0 + l1, vref * (1.f / kPStepTop), 0.f);
                 mbar_arrive(&sm.tfull[t % kPMeta]);
@@ -574,7 +585,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             for (int rr = 0; rr < 32; rr += RPI) {
                 const int rl = row - lane + rr + lane / PIECES, sl = ls - lane + rr + lane / PIECES, p = lane % PIECES;
                 if (sl >= nslots) break;
-                const int s2 = slot0 + sl, t2 = s2 / G;
+                const int s2 = slot0 + sl, t2 = row_of(s2);
                 T *y = reinterpret_cast<T *>(a.out.p) + (long long)(row0 + t2) * a.out.row_stride +
                        (long long)(kvh * G + s2 - t2 * G) * a.out.head_stride + dim0 + p * E;
                 const Vec<T, E> u = *reinterpret_cast<const Vec<T, E> *>(piece_at(rl, p));
