@@ -42,9 +42,9 @@ __device__ __forceinline__ unsigned pack4(int a, int b, int c, int d) {
 // [l*D, l*D + D) of the page's 16 tokens, so the block's maximum is one warp
 // reduction and nothing is read twice.  Bound by the rows' bytes for prompts,
 // by the chain of dependent loads for a single token.
-template <int HD, int TYPE>
-__global__ void __launch_bounds__(kKv8Warps * 32) kv8_append_kernel(Kv8 c, Kv8Rows r, Rows k, Rows v, int pages_per_seq,
-                                                                   int vec) {
+template <int HD, int TYPE, bool VEC>
+__global__ void __launch_bounds__(kKv8Warps * 32) kv8_append_kernel(Kv8 c, Kv8Rows r, Rows k, Rows v,
+                                                                   int pages_per_seq) {
     using T = typename OType<TYPE>::T;
     constexpr int D = HD / 32;
     const int lane = threadIdx.x & 31;
@@ -66,17 +66,14 @@ __global__ void __launch_bounds__(kKv8Warps * 32) kv8_append_kernel(Kv8 c, Kv8Ro
     int8_t *dst = (is_v ? c.v : c.k) + blk * (kPage * HD);
     float x[kPage][D];
     unsigned top = 0;  // |x| as integers: NaN and infinity order above every finite value
+    // slots without a new token load a neighbour's: a condition around a load would be waited for
 #pragma unroll
-    for (int t = 0; t < kPage; ++t) {
-        if (t >= lo && t < hi) {
-            load_n<D>(x0 + (long long)(row0 + p0 + t - past) * src.row_stride, vec, x[t]);
+    for (int t = 0; t < kPage; ++t)
+        load_n<D>(x0 + (long long)(row0 + p0 + min(max(t, lo), hi - 1) - past) * src.row_stride, VEC, x[t]);
 #pragma unroll
-            for (int d = 0; d < D; ++d) top = max(top, __float_as_uint(x[t][d]) & 0x7fffffffu);
-        } else {
+    for (int t = 0; t < kPage; ++t)
 #pragma unroll
-            for (int d = 0; d < D; ++d) x[t][d] = 0.f;
-        }
-    }
+        for (int d = 0; d < D; ++d) top = max(top, __float_as_uint(x[t][d]) & 0x7fffffffu);
     const float was = lo > 0 ? *scale : 0.f;
     top = __reduce_max_sync(0xffffffffu, top);
     const float amax = __uint_as_float(top);
@@ -127,9 +124,9 @@ __global__ void __launch_bounds__(kKv8Warps * 32) kv8_append_kernel(Kv8 c, Kv8Ro
 }
 
 // The values the pages stand for: the same split, one warp per block.
-template <int HD, int TYPE>
-__global__ void __launch_bounds__(kKv8Warps * 32) kv8_read_kernel(Kv8 c, Kv8Rows r, Rows k, Rows v, int pages_per_seq,
-                                                                 int vec) {
+template <int HD, int TYPE, bool VEC>
+__global__ void __launch_bounds__(kKv8Warps * 32) kv8_read_kernel(Kv8 c, Kv8Rows r, Rows k, Rows v,
+                                                                 int pages_per_seq) {
     using T = typename OType<TYPE>::T;
     constexpr int D = HD / 32;
     const int lane = threadIdx.x & 31;
@@ -166,7 +163,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32) kv8_read_kernel(Kv8 c, Kv8Rows
 #pragma unroll
             for (int d = 0; d < D; ++d) y[d] = __fmul_rn((float)u.v[d], s);
         }
-        store_n<D>(y0 + (long long)(row0 + p0 + t - past) * dst.row_stride, vec, y);
+        store_n<D>(y0 + (long long)(row0 + p0 + t - past) * dst.row_stride, VEC, y);
     }
 }
 
@@ -177,7 +174,8 @@ cudaError_t launch_kv8_append(const Kv8 &c, const Kv8Rows &r, const Rows &k, con
     const int vec = rows_vec(k, c.head_dim / 32) && rows_vec(v, c.head_dim / 32);
     count_launch();
     return kv8_dispatch(c.head_dim, k.type, [&](auto hd, auto type) {
-        kv8_append_kernel<hd, type><<<grid, kKv8Warps * 32, 0, st>>>(c, r, k, v, pages, vec);
+        if (vec) kv8_append_kernel<hd, type, true><<<grid, kKv8Warps * 32, 0, st>>>(c, r, k, v, pages);
+        else kv8_append_kernel<hd, type, false><<<grid, kKv8Warps * 32, 0, st>>>(c, r, k, v, pages);
         return cudaGetLastError();
     });
 }
@@ -189,7 +187,8 @@ cudaError_t launch_kv8_read(const Kv8 &c, const Kv8Rows &r, const Rows &k, const
     const int vec = rows_vec(k, c.head_dim / 32) && rows_vec(v, c.head_dim / 32);
     count_launch();
     return kv8_dispatch(c.head_dim, k.type, [&](auto hd, auto type) {
-        kv8_read_kernel<hd, type><<<grid, kKv8Warps * 32, 0, st>>>(c, r, k, v, pages, vec);
+        if (vec) kv8_read_kernel<hd, type, true><<<grid, kKv8Warps * 32, 0, st>>>(c, r, k, v, pages);
+        else kv8_read_kernel<hd, type, false><<<grid, kKv8Warps * 32, 0, st>>>(c, r, k, v, pages);
         return cudaGetLastError();
     });
 }

@@ -108,6 +108,17 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// 16 bytes global -> shared, past L1
+__device__ __forceinline__ void cp16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// all but the last N groups of this thread have arrived
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Most CTAs of a cluster that the operators use (more than 8 is opt-in).
 constexpr int kMaxCluster = 16;
 
@@ -152,6 +163,15 @@ template <class T, int N>
 struct alignas(sizeof(T) * N) Vec {
     T v[N];
 };
+
+// Eight elements from 16-byte aligned memory, 16 bytes an access.
+template <class T>
+__device__ __forceinline__ void load_raw(const T *p, Vec<T, 8> &x) {
+    constexpr int E = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8 / E; ++i)
+        *reinterpret_cast<Vec<T, E> *>(&x.v[i * E]) = *reinterpret_cast<const Vec<T, E> *>(p + i * E);
+}
 
 // N consecutive elements, as one access where the rows' alignment allows it
 // (vec: base and strides are multiples of N elements).

@@ -119,17 +119,6 @@ struct DecodeSmem {
     float2 ml[kMaxCluster][SLOTS];
 };
 
-// 16 bytes global -> shared, past L1
-__device__ __forceinline__ void cp16(void *dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// all but the last N groups of this thread have arrived
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // Where byte x (16-byte aligned) of a page's keys lies in shared memory: rows
 // of 128 bytes swap their halves in odd tokens, so that the 16-byte reads of
 // two tokens' 64 bytes meet all banks.

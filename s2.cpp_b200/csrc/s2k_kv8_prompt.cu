@@ -21,18 +21,19 @@
 // up to 128 slots, and f32 rows: both groups have the same 128 slots and take
 // alternate steps.
 //
-// Rounding, f16 / bf16 rows.  Q is f16 after a power of two per slot (exact but
-// for elements 2^-28 below the slot's largest).  P is f16, relative to a
-// reference within 2^8 of the running maximum, times the blocks' value scales
-// relative to a power of two above the largest seen: 2^15 at most, f16's full
-// precision down to 2^-29 of that.  O stays in TMEM (f32) and is rescaled only
-// when a reference moves: in a row's first steps and rarely after.
+// Rounding, f16 / bf16 rows.  Q is used as it is, with K in its type (int8 is
+// exact in bf16 too).  P is f16, relative to a reference within 2^8 of the
+// running maximum, times the blocks' value scales relative to a power of two
+// above the largest seen: 2^15 at most, f16's full precision down to 2^-29 of
+// that.  O stays in TMEM (f32) and is rescaled only when a reference moves: in a
+// row's first steps and rarely after.
 //
-// f32 rows.  Q and P are two f16 operands each, rounded and left over: twice the
-// products for 22 bits.  Sums in TMEM lose a little at every addition (they are
-// cut, not rounded), which over a long context would show in f32: each step's
-// O is taken out and added in registers, half of the dimensions by each group,
-// with the step's own maximum and value scale as its reference.
+// f32 rows.  Q (after a power of two per slot) and P are two f16 operands each,
+// rounded and left over: twice the products for 22 bits.  Sums in TMEM lose a
+// little at every addition (they are cut, not rounded), which over a long
+// context would show in f32: each step's O is taken out and added in registers,
+// half of the dimensions by each group, with the step's own maximum and value
+// scale as its reference.
 #include "s2k_common.cuh"
 #include "s2k_kv8.h"
 #include "s2k_tc.cuh"
@@ -57,7 +58,7 @@ struct PromptSmem {
     alignas(1024) uint8_t q[2][NC][kPM * 128];  // f32: rounded, left over; else the groups'
     alignas(1024) uint8_t k[2][NC][kPM * 128];
     alignas(1024) uint8_t v[2][2][HD * 128];
-    float qmul[2][kPM];
+    float qmul[kPM];
     struct Meta {
         float ks[kPPages], vs[kPPages];
         int p0[kPPages];
@@ -70,10 +71,10 @@ struct PromptSmem {
     uint32_t tmem;
 };
 
-// kind::f16: D f32, A and B f16, K-major, M = 128
-template <int N>
+// kind::f16: D f32, A and B f16 (or both bf16), K-major, M = 128
+template <int N, bool BF16 = false>
 constexpr uint32_t prompt_idesc() {
-    return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kPM >> 4) << 24);
+    return (1u << 4) | (BF16 ? 1u << 7 | 1u << 10 : 0) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kPM >> 4) << 24);
 }
 // An operand's descriptor (sw128_desc) by its low word: the high word is the
 // same for all, and 64-bit sums per product kept the issuing lane behind the
@@ -112,6 +113,17 @@ __device__ __forceinline__ void cvt_i8x4(uint32_t w, uint32_t &a, uint32_t &b) {
     uint32_t lo = __byte_perm(w, 0x64646464u, 0x4140), hi = __byte_perm(w, 0x64646464u, 0x4342);
     const __half2 l = __hsub2(*reinterpret_cast<__half2 *>(&lo), bias);
     const __half2 h = __hsub2(*reinterpret_cast<__half2 *>(&hi), bias);
+    a = *reinterpret_cast<const uint32_t *>(&l);
+    b = *reinterpret_cast<const uint32_t *>(&h);
+}
+// The same to bf16: with m = q mod 128, 128 + m has all its bits in bf16, and q is that less 128, or less 256 where q is
+// negative: 128 with q's sign bit as its lowest exponent bit.
+__device__ __forceinline__ void cvt_i8x4_bf16(uint32_t w, uint32_t &a, uint32_t &b) {
+    const uint32_t m = w & 0x7f7f7f7fu, n = w & 0x80808080u;
+    uint32_t x[4] = {__byte_perm(m, 0x43434343u, 0x4140), __byte_perm(n, 0x43434343u, 0x4140),
+                     __byte_perm(m, 0x43434343u, 0x4342), __byte_perm(n, 0x43434343u, 0x4342)};
+    const __nv_bfloat162 l = __hsub2(*reinterpret_cast<__nv_bfloat162 *>(&x[0]), *reinterpret_cast<__nv_bfloat162 *>(&x[1]));
+    const __nv_bfloat162 h = __hsub2(*reinterpret_cast<__nv_bfloat162 *>(&x[2]), *reinterpret_cast<__nv_bfloat162 *>(&x[3]));
     a = *reinterpret_cast<const uint32_t *>(&l);
     b = *reinterpret_cast<const uint32_t *>(&h);
 }
@@ -219,10 +231,15 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 for (int u = 0; u < U; ++u) x[e][u] = __ldg(p + u * 32);
             }
         };
-        auto put = [&](uint8_t *buf, int row, int piece, uint32_t w0, uint32_t w1) {
+        auto put = [&](uint8_t *buf, int row, int piece, uint32_t w0, uint32_t w1, bool bf16 = false) {
             uint4 h;
-            cvt_i8x4(w0, h.x, h.y);
-            cvt_i8x4(w1, h.z, h.w);
+            if (bf16) {
+                cvt_i8x4_bf16(w0, h.x, h.y);
+                cvt_i8x4_bf16(w1, h.z, h.w);
+            } else {
+                cvt_i8x4(w0, h.x, h.y);
+                cvt_i8x4(w1, h.z, h.w);
+            }
             *reinterpret_cast<uint4 *>(buf + swz(row, piece)) = h;
         };
         int pg[2], own = look_up(0), next = look_up(1), later;
@@ -255,8 +272,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                     uint8_t *buf = sm.k[s][x / 4];
                     const int flip = x / 4 & 1;
                     const uint4 w = kr[e][u];
-                    put(buf, row, 2 * (x % 4) + flip, flip ? w.z : w.x, flip ? w.w : w.y);
-                    put(buf, row, 2 * (x % 4) + 1 - flip, flip ? w.x : w.z, flip ? w.y : w.w);
+                    put(buf, row, 2 * (x % 4) + flip, flip ? w.z : w.x, flip ? w.w : w.y, TYPE == OT_BF16);
+                    put(buf, row, 2 * (x % 4) + 1 - flip, flip ? w.x : w.z, flip ? w.y : w.w, TYPE == OT_BF16);
                 }
             fence_proxy_async_smem();
             __syncwarp();
@@ -297,10 +314,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 const uint32_t d = tmem + w * kPM;
                 const uint32_t q = !split && w ? q1 : q0, k = desc_low(sm.k[s][0]);
 #pragma unroll
-                for (int x = 0; x < 4 * NC; ++x) mma_ss(d, q + at(x, kPM * 128), k + at(x, kPM * 128), prompt_idesc<kPM>(), x != 0);
+                for (int x = 0; x < 4 * NC; ++x) mma_ss(d, q + at(x, kPM * 128), k + at(x, kPM * 128), prompt_idesc<kPM, TYPE == OT_BF16>(), x != 0);
                 if (wide) {
 #pragma unroll
-                    for (int x = 0; x < 4 * NC; ++x) mma_ss(d, q1 + at(x, kPM * 128), k + at(x, kPM * 128), prompt_idesc<kPM>(), 1);
+                    for (int x = 0; x < 4 * NC; ++x) mma_ss(d, q1 + at(x, kPM * 128), k + at(x, kPM * 128), prompt_idesc<kPM, TYPE == OT_BF16>(), 1);
                 }
                 mma_commit(&sm.sfull[w]);
                 if (split || w) mma_commit(&sm.kempty[s]);
@@ -335,41 +352,68 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
     } else {
         // ---------------- softmax: one row per thread ----------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
-        // queries -> f16 operands, a warp eight slots at a time
+        // queries: a lane eight dims, LR lanes a slot
         {
-            constexpr int E = HD / 32, B = 8;
-            const float sign = a.scale < 0.f ? -1.f : 1.f;
-            const int dim = lane * E;
-            for (int s0 = (warp - 8) * B; s0 < (nslots > kPM ? 2 * kPM : kPM); s0 += 8 * B) {
-                float x[B][E];
+            constexpr int LR = HD / 8, RW = 32 / LR;
+            const int dim = lane % LR * 8, all = nslots > kPM ? 2 * kPM : kPM;
+            auto from = [&](int s) {
+                const int st = slot0 + min(s, nslots - 1), row = row_of(st);
+                return reinterpret_cast<const T *>(a.q.p) + (long long)(row0 + row) * a.q.row_stride +
+                       (long long)(kvh * G + st - row * G) * a.q.head_stride + dim;
+            };
+            if constexpr (!wide) {  // as they are
+                for (int s = (warp - 8) * RW + lane / LR; s < all; s += 8 * RW) {
+                    uint8_t *to = &sm.q[s / kPM][dim / 64][swz(s % kPM, dim % 64 / 8)];
+                    const T *p = from(s);
+                    if (vec_q) {
+                        cp16(to, p);
+                    } else {
+                        Vec<T, 8> u;
 #pragma unroll
-                for (int i = 0; i < B; ++i) {
-                    const int st = slot0 + min(s0 + i, nslots - 1), row = row_of(st);
-                    load_n<E>(reinterpret_cast<const T *>(a.q.p) + (long long)(row0 + row) * a.q.row_stride +
-                                  (long long)(kvh * G + st - row * G) * a.q.head_stride + dim,
-                              vec_q, x[i]);
+                        for (int e = 0; e < 8; ++e) u.v[e] = p[e];
+                        *reinterpret_cast<Vec<T, 8> *>(to) = u;
+                    }
                 }
+                cp_commit();
+                cp_wait<0>();
+            } else {  // -> f16 and what that leaves over
+                constexpr int B = 4;
+#pragma unroll 1
+                for (int s0 = (warp - 8) * RW * B + lane / LR; s0 < all; s0 += 8 * RW * B) {
+                    Vec<T, 8> raw8[B];
+                    // one branch around all loads: with one around each they are waited for one by one
+                    if (vec_q) {
 #pragma unroll
-                for (int i = 0; i < B; ++i) {
-                    const int s = s0 + i;
-                    unsigned top = 0;
+                        for (int i = 0; i < B; ++i) load_raw(from(s0 + i * RW), raw8[i]);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(x[i][e]) & 0x7fffffffu);
-                    top = __reduce_max_sync(kAll, top);
-                    // 2^-e brings the slot's largest to 2^13 .. 2^14
-                    const int e2 = max((int)(top >> 23) - 127, -112) - 13;
-                    const float down = sign * __int_as_float((127 - e2) << 23);
-                    if (lane == 0)
-                        sm.qmul[s / kPM][s % kPM] =
-                            top >= 0x7f800000u ? NAN : fabsf(a.scale) * 1.44269504f * __int_as_float((e2 + 127) << 23);
-                    const int at = swz(s % kPM, dim % 64 / 8) + dim % 8 * 2;
+                        for (int i = 0; i < B; ++i)
 #pragma unroll
-                    for (int e = 0; e < E / 2; ++e) {
-                        const uint32_t h = half2_bits(x[i][2 * e] * down, x[i][2 * e + 1] * down);
-                        *reinterpret_cast<uint32_t *>(&sm.q[s / kPM][dim / 64][at + 4 * e]) = h;
-                        if (wide)
-                            *reinterpret_cast<uint32_t *>(&sm.q[1][dim / 64][at + 4 * e]) =
-                                left_over(x[i][2 * e] * down, x[i][2 * e + 1] * down, h);
+                            for (int e = 0; e < 8; ++e) raw8[i].v[e] = from(s0 + i * RW)[e];
+                    }
+#pragma unroll
+                    for (int i = 0; i < B; ++i) {
+                        const int s = s0 + i * RW;
+                        unsigned top = 0;  // NaN and infinity order above as integers
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(to_f(raw8[i].v[e])) & 0x7fffffffu);
+#pragma unroll
+                        for (int o = 1; o < LR; o <<= 1) top = max(top, __shfl_xor_sync(kAll, top, o));
+                        // 2^-e brings the slot's largest to 2^13 .. 2^14
+                        const int e2 = max((int)(top >> 23) - 127, -112) - 13;
+                        const float down = __int_as_float((127 - e2) << 23);
+                        if (dim == 0)
+                            sm.qmul[s] = top >= 0x7f800000u ? NAN : a.scale * 1.44269504f * __int_as_float((e2 + 127) << 23);
+                        uint32_t h[4], lo[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float x0 = to_f(raw8[i].v[2 * e]) * down, x1 = to_f(raw8[i].v[2 * e + 1]) * down;
+                            h[e] = half2_bits(x0, x1);
+                            lo[e] = left_over(x0, x1, h[e]);
+                        }
+                        const int at = swz(s, dim % 64 / 8);
+                        *reinterpret_cast<uint4 *>(&sm.q[0][dim / 64][at]) = make_uint4(h[0], h[1], h[2], h[3]);
+                        *reinterpret_cast<uint4 *>(&sm.q[1][dim / 64][at]) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
                 }
             }
@@ -383,7 +427,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
         // positions of the warp's rows
         const int s_lo = slot0 + min(ls - lane, nslots - 1), s_hi = slot0 + min(ls - lane + 31, nslots - 1);
         const int p_min = past + row_of(s_lo), p_max = past + row_of(s_hi);
-        const float smul = sm.qmul[split ? 0 : w][row];
+        const float smul = wide ? sm.qmul[row] : a.scale * 1.44269504f;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t S = tmem + lanes + w * kPM, O = tmem + lanes + 2 * kPM + w * kPM;
         float ref = -INFINITY, l = 0.f, vref = 7.8886090522101181e-31f;
@@ -437,7 +481,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 hi = max(hi, m.p0[i]);
                 vmax = fmaxf(vmax, m.vs[i]);
             }
-            const bool edge = hi + kPage - 1 > p_min || (a.window && lo <= p_max - a.window && hi + kPage > a.sinks);
+            const bool edge = hi + kPage - 1 > p_min || (a.window && lo <= p_max - a.window && hi + kPage > a.sinks) ||
+                              a.scale < 0.f;  // the largest product is not the largest score's
             // bit i: the row sees token i of page pg
             auto below = [](long long n) { return n <= 0 ? 0u : n >= kPage ? 0xffffu : (1u << (int)n) - 1u; };
             auto seen = [&](int pg) {
@@ -449,6 +494,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             // the step's largest score.  Loops stay rolled: unrolled, with the next columns' loads ahead, they took twice
             // as long (the instruction cache serves ten warps in five places).
             float mx = -INFINITY;
+            uint32_t any = !edge;
             if (!edge) {
 #pragma unroll 1
                 for (int ch = 0; ch < 4; ++ch) {
@@ -474,12 +520,13 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                     const uint32_t bits = seen(pg);
                     const float ks = m.ks[pg] * smul;
                     if (bits) vmax = fmaxf(vmax, m.vs[pg]);
-                    float top = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < kPage; ++i) top = fmaxf(top, bits >> i & 1 ? __int_as_float(y[i]) : -INFINITY);
-                    if (top > -INFINITY) mx = fmaxf(mx, top * ks);
+                    for (int i = 0; i < kPage; ++i) mx = fmaxf(mx, bits >> i & 1 ? __int_as_float(y[i]) * ks : -INFINITY);
+                    any |= bits;
                 }
             }
+            // keys in view and no number among their scores: an infinite or NaN query or scale
+            const float odd = any && mx == -INFINITY ? NAN : 0.f;
             // a power of two from vmax on
             const float v2 = __uint_as_float((__float_as_uint(vmax) + 0x7fffffu) & 0x7f800000u);
             if (wide) {
@@ -508,7 +555,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             }
             const float base = ref == -INFINITY ? 0.f : ref;
             const float vmul = (wide ? kPStepTop : kPTop) / vref;
-            float l0 = 0.f, l1 = 0.f;
+            float l0 = odd, l1 = 0.f;
             auto weights = [&](int ch, const int(&y)[32], auto masked) {
                 uint32_t hi16[16], lo16[16];
 #pragma unroll
@@ -703,7 +750,7 @@ cudaError_t launch_kv8_prompt(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, 
     const long long tiles = (slots + per - 1) / per;
     if (slots > 0x7fffffffLL || tiles * r.n_seqs > 0x7fffffffLL) return cudaErrorInvalidValue;
     const dim3 grid((unsigned)(tiles * r.n_seqs), c.n_kv_heads);
-    const int vec_q = rows_vec(a.q, c.head_dim / 32), vec_out = rows_vec(a.out, a.out.type == OT_F32 ? 4 : 8);
+    const int vec_q = rows_vec(a.q, a.q.type == OT_F32 ? 4 : 8), vec_out = rows_vec(a.out, a.out.type == OT_F32 ? 4 : 8);
     count_launch();
     return kv8_dispatch(c.head_dim, a.q.type, [&](auto h, auto t) {
         kv8_prompt_kernel<h, t><<<grid, kPThreads, prompt_smem<h>(), st>>>(c, r, a, vec_q, vec_out);

@@ -221,6 +221,25 @@ def test_attend_hidden_blocks_may_hold_anything(rows, past, typ):
     assert torch.isnan(c.cache.attend(c.layer, q, *c.args, window=64, sinks=20, **c.kw)).all()
 
 
+@pytest.mark.parametrize("rows", [[2], [90]])
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+def test_attend_negative_scale_and_odd_queries(rows, typ):
+    """A scale below 0; rows whose scores are all -inf, +inf or NaN are NaN, their neighbours sound."""
+    c = Call(rows, [150], 8, 2, 64, typ)
+    q = c.heads(8)
+    c.check_attend(q, c.cache.attend(c.layer, q, *c.args, scale=-0.2, **c.kw), scale=-0.2)
+    good = c.cache.attend(c.layer, q, *c.args, **c.kw)
+    c.cache.k[:, c.layer, :, :, 5] = 3  # one dim of one sign
+    same = c.cache.attend(c.layer, q, *c.args, **c.kw)
+    odd = q.clone()
+    odd[0, 0, 5], odd[0, 1, 5], odd[1, 2, 5] = float("inf"), -float("inf"), float("nan")
+    out = c.cache.attend(c.layer, odd, *c.args, **c.kw)
+    for r, h in ((0, 0), (0, 1), (1, 2)):
+        assert torch.isnan(out[r, h]).all()
+        out[r, h] = same[r, h]
+    assert torch.equal(out, same) and not torch.equal(good, same)
+
+
 @pytest.mark.parametrize("rows", [1, 90])
 def test_attend_far_scores_scales_and_not_a_number(rows):
     """Queries and blocks of very different size, a row of zeros, a NaN and an infinite row beside sound ones."""
