@@ -172,6 +172,18 @@ S2K_API void *s2k_model_stream(s2k_model *m);
 /* SlowARModel::init_kv_cache (src/s2_model.cpp:717-765): a sequence owning a
  * paged f16 KV cache (16-token pages) for up to max_seq_len positions. */
 S2K_API s2k_status s2k_seq_create(s2k_model *m, int32_t max_seq_len, s2k_seq **out);
+/* The same with the KV cache in 8 bits (an s2k_kv8 of its own: 1.002 bytes per
+ * value instead of 2) and, with window > 0, attention to the last `window`
+ * positions and the first `sinks` ones only.  s2k_eval, s2k_eval_logprobs,
+ * s2k_generate(_device), s2k_seq_load_kv, s2k_seq_reset and s2k_seq_free take
+ * such a sequence; s2k_seq_begin, s2k_batch_frame and the profiling hooks need
+ * an f16 one (S2K_ERR_UNSUPPORTED / S2K_ERR_STATE).  A call's own keys and
+ * values are read back from the cache like the past, so logits differ from
+ * those over an f16 cache by the rounding of s2k_kv8_append, and a prompt given
+ * in one call rounds otherwise than one given token by token.  Its steps and
+ * frames run kernel by kernel instead of as one persistent kernel. */
+S2K_API s2k_status s2k_seq_create_kv8(s2k_model *m, int32_t max_seq_len, int32_t window, int32_t sinks,
+                                      s2k_seq **out);
 /* SlowARModel::reset (src/s2_model.cpp:767-769): n_past = 0. */
 S2K_API s2k_status s2k_seq_reset(s2k_seq *s);
 /* SlowARModel::clear_kv_cache (src/s2_model.cpp:771-787). */
@@ -192,6 +204,21 @@ S2K_API s2k_status s2k_seq_load_kv(s2k_seq *s, const uint16_t *k, const uint16_t
  * host buffers (either may be NULL). */
 S2K_API s2k_status s2k_eval(s2k_model *m, s2k_seq *s, const int32_t *flat_tokens,
                             int32_t n_tokens, float *hidden_out, float *logits_out);
+
+/* How likely the given tokens are (no reference counterpart): s2k_eval of
+ * n_tokens tokens that returns, from the logits of every position instead of
+ * the last one's, in host arrays (each may be NULL but for the top ones with
+ * n_top > 0):
+ *   logprob [n_tokens - 1]          of the main token t + 1 after tokens 0 .. t
+ *   entropy [n_tokens]              of each position's distribution, in nats
+ *   top_ids, top_logprobs [n_tokens][n_top]  its n_top (0 .. S2K_LOGPROBS_MAX_TOP)
+ *                                   most likely main tokens, as s2k_logprobs
+ * n_past advances as in s2k_eval, so long texts can be given in parts (the
+ * first token of a part is then scored by the top alternatives or entropy of
+ * the part before only). */
+S2K_API s2k_status s2k_eval_logprobs(s2k_model *m, s2k_seq *s, const int32_t *flat_tokens, int32_t n_tokens,
+                                     int32_t n_top, float *logprob, float *entropy, int32_t *top_ids,
+                                     float *top_logprobs);
 
 /* SlowARModel::fast_decode (src/s2_model.cpp:1099-1255): hidden [embedding_length],
  * prefix [n_prefix] codebook values, n_prefix < num_codebooks; logits_out

@@ -329,7 +329,31 @@ cudaError_t run_stack(s2k_model *m, const StackCall &c) {
         a.out = w.attn;
         a.done = c.done;
         a.err = m->d_err;
-        if ((e = launch_attention(a, st))) return e;
+        if (c.kv8) {
+            // 8-bit cache: this call's K/V go into it first and are read back from it, like the past
+            Kv8 cache = c.kv8->kv8;
+            cache.layer = (int)il;
+            Kv8Rows r;
+            r.n_seqs = 1;
+            r.n_rows = r.max_rows = c.T;
+            r.table_ld = c.kv8->n_pages;
+            r.past = c.pos_base;
+            r.table = c.kv8->block_table;
+            r.err = r.block = m->d_err;
+            r.done = c.done;
+            const long long kvs = (long long)Hkv * hd;
+            if ((e = launch_kv8_append(cache, r, Rows{q.kcur, OT_F32, kvs, hd}, Rows{q.vcur, OT_F32, kvs, hd}, st))) return e;
+            Kv8Attn v;
+            v.q = Rows{w.qkv, OT_F32, qkvs, hd};
+            v.out = Rows{w.attn, OT_F32, (long long)H * hd, hd};
+            v.n_heads = H;
+            v.scale = a.scale;
+            v.window = c.kv8->window;
+            v.sinks = c.kv8->sinks;
+            if ((e = launch_kv8_attend(cache, r, v, st))) return e;
+        } else if ((e = launch_attention(a, st))) {
+            return e;
+        }
 
         GemvArgs o = g;
         o.w = &L.wo;
@@ -371,7 +395,7 @@ cudaError_t run_stack(s2k_model *m, const StackCall &c) {
 
 // Slow step over T tokens already in `tokens_dev` ([T][ncb+1]): embedding,
 // 36 layers, final norm + tied LM head on the last token, n_past += T.
-cudaError_t enqueue_slow(s2k_model *m, s2k_seq *s, int T, const int *tokens_dev, const int *done) {
+cudaError_t enqueue_slow_layers(s2k_model *m, s2k_seq *s, int T, const int *tokens_dev, const int *done) {
     const s2k_hparams &hp = m->hp;
     cudaStream_t st = m->stream;
     cudaError_t e;
@@ -398,10 +422,18 @@ cudaError_t enqueue_slow(s2k_model *m, s2k_seq *s, int T, const int *tokens_dev,
     c.pos_base = &s->dev->state.n_past;
     c.pos_add = 0;
     c.cur_base = 0;
-    c.kv = s->kv();
+    if (s->is_kv8()) c.kv8 = s;
+    else c.kv = s->kv();
     c.max_keys = m->sw.L;
     c.done = done;
-    if ((e = run_stack(m, c))) return e;
+    return run_stack(m, c);
+}
+
+cudaError_t enqueue_slow(s2k_model *m, s2k_seq *s, int T, const int *tokens_dev, const int *done) {
+    const s2k_hparams &hp = m->hp;
+    cudaStream_t st = m->stream;
+    cudaError_t e;
+    if ((e = enqueue_slow_layers(m, s, T, tokens_dev, done))) return e;
     GemvArgs hd;
     hd.w = &m->embed;
     hd.x = m->sw.x + (size_t)(T - 1) * hp.embedding_length;
@@ -848,8 +880,9 @@ s2k_status seq_publish(s2k_seq *s) {
     return S2K_OK;
 }
 
-S2K_API s2k_status s2k_seq_create(s2k_model *m, int32_t max_seq_len, s2k_seq **out) {
+static s2k_status seq_create(s2k_model *m, int32_t max_seq_len, bool kv8, int32_t window, int32_t sinks, s2k_seq **out) {
     if (!m || !out || max_seq_len <= 0) return fail(S2K_ERR_ARG, "bad argument");
+    if (window < 0 || sinks < 0) return fail(S2K_ERR_ARG, "window %d, sinks %d", window, sinks);
     if (!m->finalized) return fail(S2K_ERR_STATE, "model not finalized");
     if (max_seq_len > m->rope_slow_n)
         return fail(S2K_ERR_ARG, "max_seq_len %d exceeds context_length %d", max_seq_len, m->rope_slow_n);
@@ -865,8 +898,21 @@ S2K_API s2k_status s2k_seq_create(s2k_model *m, int32_t max_seq_len, s2k_seq **o
         s2k_seq_free(s);
         return fail(code, "s2k_seq_create: %s", what);
     };
-    if (m->alloc(&s->k, page_elems * s->n_pages) || m->alloc(&s->v, page_elems * s->n_pages))
+    if (kv8) {
+        const size_t blocks = (size_t)s->n_pages * hp.block_count * hp.head_count_kv;
+        Kv8 &c = s->kv8;
+        c.n_pages = s->n_pages;
+        c.n_layers = hp.block_count;
+        c.n_kv_heads = hp.head_count_kv;
+        c.head_dim = hp.head_dim;
+        s->window = window;
+        s->sinks = sinks;
+        if (m->alloc(&c.k, page_elems * s->n_pages) || m->alloc(&c.v, page_elems * s->n_pages) ||
+            m->alloc(&c.k_scale, blocks) || m->alloc(&c.v_scale, blocks))
+            return cleanup(S2K_ERR_OOM, "KV pages");
+    } else if (m->alloc(&s->k, page_elems * s->n_pages) || m->alloc(&s->v, page_elems * s->n_pages)) {
         return cleanup(S2K_ERR_OOM, "KV pages");
+    }
     std::vector<int> bt(s->n_pages);
     for (int i = 0; i < s->n_pages; ++i) bt[i] = i;
     if (m->alloc(&s->block_table, (size_t)s->n_pages) ||
@@ -883,6 +929,14 @@ S2K_API s2k_status s2k_seq_create(s2k_model *m, int32_t max_seq_len, s2k_seq **o
         return cleanup(S2K_ERR_CUDA, "host status mapping");
     *out = s;
     return S2K_OK;
+}
+
+S2K_API s2k_status s2k_seq_create(s2k_model *m, int32_t max_seq_len, s2k_seq **out) {
+    return seq_create(m, max_seq_len, false, 0, 0, out);
+}
+
+S2K_API s2k_status s2k_seq_create_kv8(s2k_model *m, int32_t max_seq_len, int32_t window, int32_t sinks, s2k_seq **out) {
+    return seq_create(m, max_seq_len, true, window, sinks, out);
 }
 
 S2K_API s2k_status s2k_seq_reset(s2k_seq *s) {
@@ -904,6 +958,10 @@ S2K_API void s2k_seq_free(s2k_seq *s) {
         m->release(s->k);
         m->release(s->v);
     }
+    m->release(s->kv8.k);
+    m->release(s->kv8.v);
+    m->release(s->kv8.k_scale);
+    m->release(s->kv8.v_scale);
     m->release(s->hidden);
     m->release(s->block_table);
     m->release(s->dev);
@@ -937,6 +995,20 @@ s2k_status check_tokens_host(const s2k_model *m, const int32_t *flat, int32_t T)
 
 static s2k_status ensure_eval_program(s2k_model *m, s2k_seq *s);
 
+// The call's token rows in device memory (m->tokens).
+static s2k_status upload_tokens(s2k_model *m, const int32_t *flat, int32_t T) {
+    const int n = T * (m->hp.num_codebooks + 1);
+    if (m->tokens_cap < n) {
+        m->release(m->tokens);
+        m->tokens = nullptr;
+        m->tokens_cap = 0;
+        CU(m->alloc(&m->tokens, (size_t)n));
+        m->tokens_cap = n;
+    }
+    CU(cudaMemcpyAsync(m->tokens, flat, (size_t)n * sizeof(int), cudaMemcpyHostToDevice, m->stream));
+    return S2K_OK;
+}
+
 S2K_API s2k_status s2k_eval(s2k_model *m, s2k_seq *s, const int32_t *flat, int32_t T, float *hidden_out,
                             float *logits_out) {
     if (!m || !s || !flat || T <= 0) return fail(S2K_ERR_ARG, "bad argument");
@@ -951,7 +1023,7 @@ S2K_API s2k_status s2k_eval(s2k_model *m, s2k_seq *s, const int32_t *flat, int32
     if (rc) return rc;
     const int stride = m->hp.num_codebooks + 1;
     bool on_mega = false;
-    if (T == 1 && !s->pooled) {
+    if (T == 1 && !s->pooled && !s->is_kv8()) {
         // one token: the whole step as one persistent-kernel launch
         rc = ensure_eval_program(m, s);
         if (rc) return rc;
@@ -963,19 +1035,99 @@ S2K_API s2k_status s2k_eval(s2k_model *m, s2k_seq *s, const int32_t *flat, int32
         CU(launch_mega(s->eval_ops, s->eval_len, 1, s->eval_ctl, nullptr, m->d_err, m->num_sms, m->stream, m->d_epoch,
                        s->eval_q8));
     } else {
-        if (m->tokens_cap < T * stride) {
-            m->release(m->tokens);
-            m->tokens = nullptr;
-            CU(m->alloc(&m->tokens, (size_t)T * stride));
-            m->tokens_cap = T * stride;
-        }
-        CU(cudaMemcpyAsync(m->tokens, flat, (size_t)T * stride * sizeof(int), cudaMemcpyHostToDevice, m->stream));
+        rc = upload_tokens(m, flat, T);
+        if (rc) return rc;
         CU(enqueue_slow(m, s, T, m->tokens, nullptr));
     }
     if (hidden_out)
         CU(cudaMemcpyAsync(hidden_out, m->hidden, (size_t)m->hp.embedding_length * 4, cudaMemcpyDeviceToHost, m->stream));
     if (logits_out)
         CU(cudaMemcpyAsync(logits_out, m->logits, (size_t)m->hp.vocab_size * 4, cudaMemcpyDeviceToHost, m->stream));
+    CU(cudaStreamSynchronize(m->stream));
+    rc = check_err_word(m);
+    if (rc) return rc;
+    s->n_past += T;
+    return S2K_OK;
+}
+
+// Rows of logits of s2k_eval_logprobs at once (40 MB at S2 Pro's vocabulary).
+constexpr int kLogprobRows = 64;
+
+S2K_API s2k_status s2k_eval_logprobs(s2k_model *m, s2k_seq *s, const int32_t *flat, int32_t T, int32_t n_top,
+                                     float *logprob, float *entropy, int32_t *top_ids, float *top_logprobs) {
+    if (!m || !s || !flat || T <= 0) return fail(S2K_ERR_ARG, "bad argument");
+    if (!m->finalized) return fail(S2K_ERR_STATE, "model not finalized");
+    if (s->m != m) return fail(S2K_ERR_ARG, "sequence belongs to another model");
+    const s2k_hparams &hp = m->hp;
+    if (n_top < 0 || n_top > S2K_LOGPROBS_MAX_TOP || n_top > hp.vocab_size)
+        return fail(S2K_ERR_ARG, "%d alternatives (at most %d)", n_top, S2K_LOGPROBS_MAX_TOP);
+    if (n_top > 0 && (!top_ids || !top_logprobs)) return fail(S2K_ERR_ARG, "NULL top outputs");
+    if (s->n_past + T > s->max_seq_len)
+        return fail(S2K_ERR_KV_FULL, "KV cache overflow (%d + %d > %d)", s->n_past, T, s->max_seq_len);
+    s2k_status rc = check_tokens_host(m, flat, T);
+    if (rc) return rc;
+    if (cuda_set(m->device)) return fail(S2K_ERR_CUDA, "cudaSetDevice failed");
+    rc = ensure_slow_work(m, T, s->max_seq_len);
+    if (rc) return rc;
+    const int rows = std::min(T, kLogprobRows);
+    if (m->lp_rows < rows) {
+        m->release(m->lp_logits);
+        m->lp_logits = nullptr;
+        m->lp_rows = 0;
+        CU(m->alloc(&m->lp_logits, (size_t)rows * hp.vocab_size));
+        m->lp_rows = rows;
+    }
+    // per token: log probability, entropy, alternatives; next token, alternatives' ids
+    if (m->lp_tokens < T) {
+        m->release(m->lp_out);
+        m->release(m->lp_ids);
+        m->lp_out = nullptr;
+        m->lp_ids = nullptr;
+        m->lp_tokens = 0;
+        CU(m->alloc(&m->lp_out, (size_t)T * (2 + S2K_LOGPROBS_MAX_TOP)));
+        CU(m->alloc(&m->lp_ids, (size_t)T * (1 + S2K_LOGPROBS_MAX_TOP)));
+        m->lp_tokens = T;
+    }
+    std::vector<int32_t> next((size_t)T, -1);
+    for (int t = 0; t + 1 < T; ++t) next[t] = flat[(size_t)(t + 1) * (hp.num_codebooks + 1)];
+    rc = upload_tokens(m, flat, T);
+    if (rc) return rc;
+    CU(cudaMemcpyAsync(m->lp_ids, next.data(), (size_t)T * sizeof(int), cudaMemcpyHostToDevice, m->stream));
+    CU(enqueue_slow_layers(m, s, T, m->tokens, nullptr));
+    for (int t0 = 0; t0 < T; t0 += rows) {
+        GemvArgs g;
+        g.w = &m->embed;
+        g.x = m->sw.x + (size_t)t0 * hp.embedding_length;
+        g.ldx = hp.embedding_length;
+        g.M = std::min(rows, T - t0);
+        g.in_mode = IN_RMSNORM;
+        g.norm_w = m->norm;
+        g.eps = hp.rms_norm_eps;
+        g.y = m->lp_logits;
+        g.ldy = hp.vocab_size;
+        g.err = m->d_err;
+        CU(stack_gemm(m, m->sw, g, true, T >= kPrefillMinT));
+        LogprobArgs a;
+        a.x = m->lp_logits;
+        a.rows = g.M;
+        a.n = hp.vocab_size;
+        a.ld = hp.vocab_size;
+        a.targets = m->lp_ids + t0;
+        a.n_top = n_top;
+        a.logprob = m->lp_out + t0;
+        a.entropy = m->lp_out + T + t0;
+        a.top_ids = m->lp_ids + T + (size_t)t0 * n_top;
+        a.top_logprob = m->lp_out + 2 * (size_t)T + (size_t)t0 * n_top;
+        CU(launch_logprobs(a, m->stream));
+    }
+    CU(launch_advance(s->dev, T, nullptr, m->stream));
+    auto back = [&](void *dst, const void *src, size_t n) {
+        return dst && n ? cudaMemcpyAsync(dst, src, n * 4, cudaMemcpyDeviceToHost, m->stream) : cudaSuccess;
+    };
+    CU(back(logprob, m->lp_out, (size_t)T - 1));
+    CU(back(entropy, m->lp_out + T, (size_t)T));
+    CU(back(top_ids, m->lp_ids + T, (size_t)T * n_top));
+    CU(back(top_logprobs, m->lp_out + 2 * (size_t)T, (size_t)T * n_top));
     CU(cudaStreamSynchronize(m->stream));
     rc = check_err_word(m);
     if (rc) return rc;
@@ -1371,7 +1523,9 @@ static s2k_status ensure_frame_graph(s2k_model *m, s2k_seq *s) {
     }
     cudaGraph_t g = nullptr;
     const unsigned long long before = g_launches.load();
-    s2k_status brc = build_mega(m, s);
+    // the persistent kernel's attention reads f16 pages: an 8-bit sequence's frames run kernel by kernel
+    s->use_mega = false;
+    s2k_status brc = s->is_kv8() ? S2K_OK : build_mega(m, s);
     if (brc) return brc;
     CU(cudaStreamBeginCapture(m->stream, cudaStreamCaptureModeThreadLocal));
     cudaError_t e = s->use_mega ? enqueue_frame_mega(m, s) : enqueue_frame(m, s);
@@ -1866,7 +2020,36 @@ S2K_API s2k_status s2k_seq_load_kv(s2k_seq *s, const uint16_t *k, const uint16_t
     const size_t kvs = (size_t)Hkv * hd;
     const size_t page_elems = (size_t)L * Hkv * kPage * hd;
     const int np = (n_pos + kPage - 1) / kPage;
-    if (np > 0) {
+    if (s->is_kv8() && n_pos > 0) {
+        // rounded into the 8-bit blocks layer by layer, as one call of n_pos tokens stores them
+        CU(cudaStreamSynchronize(m->stream));
+        CU(cudaMemsetAsync(&s->dev->state, 0, sizeof(SeqState), m->stream));
+        __half *rows = nullptr;
+        CU(m->alloc(&rows, 2 * (size_t)n_pos * kvs));
+        cudaError_t e = cudaSuccess;
+        for (int l = 0; l < L && e == cudaSuccess; ++l) {
+            const size_t n = (size_t)n_pos * kvs, at = (size_t)l * n;
+            if ((e = cudaMemcpyAsync(rows, k + at, n * 2, cudaMemcpyHostToDevice, m->stream))) break;
+            if ((e = cudaMemcpyAsync(rows + n, v + at, n * 2, cudaMemcpyHostToDevice, m->stream))) break;
+            Kv8 cache = s->kv8;
+            cache.layer = l;
+            Kv8Rows r;
+            r.n_seqs = 1;
+            r.n_rows = r.max_rows = n_pos;
+            r.table_ld = s->n_pages;
+            r.past = &s->dev->state.n_past;
+            r.table = s->block_table;
+            r.err = m->d_err;
+            e = launch_kv8_append(cache, r, Rows{rows, OT_F16, (long long)kvs, hd},
+                                  Rows{rows + n, OT_F16, (long long)kvs, hd}, m->stream);
+        }
+        const cudaError_t e2 = cudaStreamSynchronize(m->stream);
+        m->release(rows);
+        CU(e);
+        CU(e2);
+        const s2k_status rc = check_err_word(m);
+        if (rc) return rc;
+    } else if (np > 0) {
         // [layer][pos][kv_head][hd] -> pages [page][layer][kv_head][slot][hd]; the
         // sequence's own block table is the identity (s2k_seq_create)
         std::vector<uint16_t> pk((size_t)np * page_elems, 0), pv((size_t)np * page_elems, 0);

@@ -335,6 +335,7 @@ S2K_API s2k_status s2k_seq_begin(s2k_model *m, s2k_seq *s, const int32_t *prompt
     if (!m || !s || !prompt || !gp || cols <= 0) return fail(S2K_ERR_ARG, "bad argument");
     if (!m->finalized) return fail(S2K_ERR_STATE, "model not finalized");
     if (s->m != m) return fail(S2K_ERR_ARG, "sequence belongs to another model");
+    if (s->is_kv8()) return fail(S2K_ERR_UNSUPPORTED, "batched frames read f16 caches");
     if (cuda_set(m->device)) return fail(S2K_ERR_CUDA, "cudaSetDevice failed");
     s2k_status rc = upload_prompt(m, s, prompt, cols);
     if (!rc) rc = ensure_codes(m, s, gp->max_new_tokens);
@@ -353,6 +354,7 @@ S2K_API s2k_status s2k_batch_frame(s2k_model *m, s2k_seq *const *seqs, int32_t n
     std::vector<s2k_seq *> live;
     for (int i = 0; i < n; ++i) {
         if (!seqs[i] || seqs[i]->m != m) return fail(S2K_ERR_ARG, "sequence %d is NULL or belongs to another model", i);
+        if (seqs[i]->is_kv8()) return fail(S2K_ERR_UNSUPPORTED, "batched frames read f16 caches");
         if (!seqs[i]->hstat->done) live.push_back(seqs[i]);
     }
     for (size_t i = 0; i < live.size(); ++i)

@@ -41,6 +41,8 @@ struct Kv8Rows {
     const int *row_start = nullptr;  // [n_seqs + 1], null: max_rows rows each
     const int *table = nullptr;      // [n_seqs][table_ld]
     int *err = nullptr;              // optional error word
+    int *block = nullptr;            // a model's error block (its wait limit), where the call is one of a model's
+    const int *done = nullptr;       // optional: nothing is done once it is set (frame loop)
 };
 
 struct Rows {
@@ -53,6 +55,7 @@ struct Rows {
 // Sequence b's rows, false (and an error bit) when what the device arrays say
 // does not fit the call: nothing of that sequence is then read or written.
 __device__ __forceinline__ bool kv8_seq(const Kv8Rows &r, int b, int &row0, int &T, int &past) {
+    if (r.done && __ldcg(r.done)) return false;
     row0 = r.row_start ? r.row_start[b] : b * r.max_rows;
     T = r.row_start ? r.row_start[b + 1] - row0 : r.max_rows;
     past = r.past[b];
@@ -60,6 +63,13 @@ __device__ __forceinline__ bool kv8_seq(const Kv8Rows &r, int b, int &row0, int 
                     past <= r.table_ld * kPage - T;
     if (!ok && r.err && threadIdx.x == 0) atomicOr(r.err, ERR_BAD_POS);
     return ok;
+}
+
+// Bounded wait on an mbarrier phase; the caller's error word has no wait limit behind it, a model's block does.
+__device__ __forceinline__ bool kv8_wait(const Kv8Rows &r, uint64_t *bar, uint32_t parity, int code) {
+    if (mbar_wait(bar, parity, r.block, code)) return true;
+    if (r.err) atomicOr(r.err, code);
+    return false;
 }
 
 // Physical page of logical page pg, -1 (and an error bit) when the table

@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             const int s = t & 1;
             fetch(c.v, pg, vr);
             later = look_up(t + 2);
-            if (t >= 2) ok = mbar_wait(&sm.kempty[s], ((t >> 1) - 1) & 1, r.err, ERR_WAIT_EMPTY);
+            if (t >= 2) ok = kv8_wait(r, &sm.kempty[s], ((t >> 1) - 1) & 1, ERR_WAIT_EMPTY);
             if (!(ok = __all_sync(kAll, ok))) break;
             if (lane < 2) {
                 typename Sm::Meta &m = sm.meta[t % kPMeta];
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             pg[1] = __shfl_sync(kAll, own, 1);
             fetch(c.k, pg, kr);
             scales(own, ks, vs);
-            if (t >= 2) ok = mbar_wait(&sm.vempty[s], ((t >> 1) - 1) & 1, r.err, ERR_WAIT_EMPTY);
+            if (t >= 2) ok = kv8_wait(r, &sm.vempty[s], ((t >> 1) - 1) & 1, ERR_WAIT_EMPTY);
             if (!(ok = __all_sync(kAll, ok))) break;
 #pragma unroll
             for (int e = 0; e < 2; ++e)
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             auto at = [](int x, int chunk) { return (uint32_t)(2 * (x % 4) + (x / 4) * (chunk >> 4)); };
             auto qk = [&](int g) {
                 const int t = split ? g : g >> 1, w = g & 1, s = t & 1;
-                if (!mbar_wait(&sm.kfull[s], (t >> 1) & 1, r.err, ERR_WAIT_FULL)) return false;
+                if (!kv8_wait(r, &sm.kfull[s], (t >> 1) & 1, ERR_WAIT_FULL)) return false;
                 tc_fence_after();
                 const uint32_t d = tmem + w * kPM;
                 const uint32_t q = !split && w ? q1 : q0, k = desc_low(sm.k[s][0]);
@@ -323,17 +323,17 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 if (split || w) mma_commit(&sm.kempty[s]);
                 return true;
             };
-            ok = mbar_wait(&sm.qfull, 0, r.err, ERR_WAIT_FULL) && qk(0);
+            ok = kv8_wait(r, &sm.qfull, 0, ERR_WAIT_FULL) && qk(0);
             if (ok && jobs > 1) ok = qk(1);
             for (int g = 0; g < jobs && ok; ++g) {
                 const int t = split ? g : g >> 1, w = g & 1, s = t & 1;
                 const uint32_t d = tmem + 2 * kPM + w * kPM, p = tmem + w * kPM;
                 const uint32_t v = desc_low(sm.v[s][0]);
-                ok = mbar_wait(&sm.vfull[s], (t >> 1) & 1, r.err, ERR_WAIT_FULL);
+                ok = kv8_wait(r, &sm.vfull[s], (t >> 1) & 1, ERR_WAIT_FULL);
                 // f32 rows: the output of two steps ago has been taken
-                if (ok && wide && g > 1) ok = mbar_wait(&sm.ofree[w], ((g >> 1) - 1) & 1, r.err, ERR_WAIT_EMPTY);
+                if (ok && wide && g > 1) ok = kv8_wait(r, &sm.ofree[w], ((g >> 1) - 1) & 1, ERR_WAIT_EMPTY);
                 for (int h = 0; h < 2 && ok; ++h) {  // 64 keys each
-                    if (!(ok = mbar_wait(&sm.pfull[w][h], (g >> 1) & 1, r.err, ERR_WAIT_FULL))) break;
+                    if (!(ok = kv8_wait(r, &sm.pfull[w][h], (g >> 1) & 1, ERR_WAIT_FULL))) break;
                     tc_fence_after();
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.qfull);
-            ok = mbar_wait(&sm.qfull, 0, r.err, ERR_WAIT_FULL);
+            ok = kv8_wait(r, &sm.qfull, 0, ERR_WAIT_FULL);
         }
         const int w = (warp >> 2) - 2, row = tid & (kPM - 1), ls = (split ? 0 : w * kPM) + row;
         const int pos = past + row_of(slot0 + min(ls, nslots - 1));
@@ -438,8 +438,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
         for (int i = 0; i < HALF; ++i) acc[i] = 0.f;
         float top_ref = -INFINITY, sum = 0.f;
         auto take = [&](int t) {  // f32 rows: adds step t's output
-            bool fine = mbar_wait(&sm.tfull[t % kPMeta], (t / kPMeta) & 1, r.err, ERR_WAIT_FULL) &&
-                        mbar_wait(&sm.odone[t & 1], (t >> 1) & 1, r.err, ERR_WAIT_FULL);
+            bool fine = kv8_wait(r, &sm.tfull[t % kPMeta], (t / kPMeta) & 1, ERR_WAIT_FULL) &&
+                        kv8_wait(r, &sm.odone[t & 1], (t >> 1) & 1, ERR_WAIT_FULL);
             if (!__all_sync(kAll, fine)) return false;
             tc_fence_after();
             const float4 z = sm.stat[t % kPMeta][row];
@@ -468,8 +468,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 continue;
             }
             const int t = split ? g : g >> 1;
-            ok = mbar_wait(&sm.mfull[t % kPMeta], (t / kPMeta) & 1, r.err, ERR_WAIT_FULL) &&
-                 mbar_wait(&sm.sfull[w], done & 1, r.err, ERR_WAIT_FULL);
+            ok = kv8_wait(r, &sm.mfull[t % kPMeta], (t / kPMeta) & 1, ERR_WAIT_FULL) &&
+                 kv8_wait(r, &sm.sfull[w], done & 1, ERR_WAIT_FULL);
             if (!(ok = __all_sync(kAll, ok))) break;
             tc_fence_after();
             const typename Sm::Meta &m = sm.meta[t % kPMeta];
@@ -657,8 +657,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             }
             store_rows(w * HALF);
         } else {
-            if (ok && done) ok = mbar_wait(&sm.odone[w], 0, r.err, ERR_WAIT_FULL);
-            if (ok && split && w) ok = mbar_wait(&sm.odone[0], 0, r.err, ERR_WAIT_FULL);  // it stores where V was
+            if (ok && done) ok = kv8_wait(r, &sm.odone[w], 0, ERR_WAIT_FULL);
+            if (ok && split && w) ok = kv8_wait(r, &sm.odone[0], 0, ERR_WAIT_FULL);  // it stores where V was
             ok = __all_sync(kAll, ok);
             if (!ok) l = NAN;
             tc_fence_after();

@@ -7,6 +7,7 @@
 #include "s2k_common.cuh"
 #include "s2k_device.h"
 #include "s2k_kernels.h"
+#include "s2k_kv8.h"
 #include "s2k_mega.h"
 
 #include <algorithm>
@@ -119,6 +120,10 @@ struct s2k_model {
     float *samp_logits = nullptr;
     int samp_cap = 0;
     int *samp_out = nullptr;
+    // s2k_eval_logprobs: logits of a chunk of rows and what is made of them
+    float *lp_logits = nullptr, *lp_out = nullptr;
+    int *lp_ids = nullptr;
+    int lp_rows = 0, lp_tokens = 0;
     // batched frames (s2k_batch.cu)
     BatchState *batch = nullptr;
 
@@ -160,6 +165,9 @@ struct s2k_seq {
     int n_past = 0;                   // host mirror
     float *hidden = nullptr;          // Slow hidden state that feeds the next Fast-AR pass (batched frames)
     bool pooled = false;              // k / v belong to a scheduler's page pool
+    Kv8 kv8;                          // an 8-bit cache instead of k / v (s2k_seq_create_kv8), with its attention's view
+    int window = 0, sinks = 0;
+    bool is_kv8() const { return kv8.k != nullptr; }
     int *codes = nullptr;             // [ncb][codes_cap]
     int codes_cap = 0;
     int *prompt = nullptr;
@@ -202,6 +210,7 @@ struct StackCall {
     int pos_add = 0;
     int cur_base = 0;
     KvPaged kv;        // Slow only
+    const s2k_seq *kv8 = nullptr;  // Slow only: the sequence with an 8-bit cache, instead of kv
     int max_keys = 0;  // upper bound of any token's key range
     const int *done = nullptr;
     // batched calls over independent sequences: per-row descriptors and the
@@ -233,6 +242,8 @@ s2k_status ensure_slow_work(s2k_model *m, int T, int L);
 cudaError_t stack_gemm(s2k_model *m, Work &w, const GemvArgs &g, bool exact, bool f16 = false);
 cudaError_t run_stack(s2k_model *m, const StackCall &c);
 cudaError_t enqueue_slow(s2k_model *m, s2k_seq *s, int T, const int *tokens_dev, const int *done);
+// its embedding and layers alone: T rows of m->sw.x
+cudaError_t enqueue_slow_layers(s2k_model *m, s2k_seq *s, int T, const int *tokens_dev, const int *done);
 s2k_status check_tokens_host(const s2k_model *m, const int32_t *flat, int32_t T);
 void fill_sample_cfg(const s2k_model *m, const s2k_gen_params *gp, int *d_codes, int codes_ld, SampleCfg *c);
 void batch_free(s2k_model *m);

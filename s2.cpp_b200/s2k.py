@@ -46,6 +46,7 @@ EXPORTED = [
     "s2k_codec_receptive_frames", "s2k_codec_decode", "s2k_codec_decode_range", "s2k_codec_decode_windowed",
     "s2k_codec_stream_create", "s2k_codec_stream_free", "s2k_codec_stream_push", "s2k_codec_stream_finish",
     "s2k_codec_stream_max_release",
+    "s2k_seq_create_kv8", "s2k_eval_logprobs",
     "s2k_kv8_append", "s2k_kv8_read", "s2k_kv8_attend", "s2k_logprobs",
 ]
 
@@ -245,6 +246,8 @@ def lib() -> ctypes.CDLL:
         "s2k_codec_stream_push": ([vp, vp, vp, ctypes.c_size_t, i64p], i32),
         "s2k_codec_stream_finish": ([vp, vp, ctypes.c_size_t, i64p], i32),
         "s2k_codec_stream_max_release": ([vp], ctypes.c_int64),
+        "s2k_seq_create_kv8": ([vp, i32, i32, i32, ctypes.POINTER(vp)], i32),
+        "s2k_eval_logprobs": ([vp, vp, vp, i32, i32, vp, vp, vp, vp], i32),
         "s2k_kv8_append": ([vp, i32, vp, vp, vp, vp], i32),
         "s2k_kv8_read": ([vp, i32, vp, vp, vp, vp], i32),
         "s2k_kv8_attend": ([vp, i32, vp, vp, vp, i32, ctypes.c_float, i32, i32, vp], i32),
@@ -430,6 +433,14 @@ class SlowARModel:
         _check(lib().s2k_seq_create(self._m, max_seq_len, ctypes.byref(self._seq)))
         self._max_seq_len = max_seq_len
 
+    def init_kv8_cache(self, max_seq_len: int, window: int = 0, sinks: int = 0) -> None:
+        """A KV cache in 8 bits, with attention to the last `window` (0: all) and the first `sinks` positions
+        (s2k_seq_create_kv8)."""
+        self.clear_kv_cache()
+        _check(lib().s2k_seq_create_kv8(self._m, max_seq_len, window, sinks, ctypes.byref(self._seq)))
+        self._max_seq_len = max_seq_len
+        self._kv8 = (window, sinks)
+
     def reset(self) -> None:
         _check(lib().s2k_seq_reset(self._seq))
 
@@ -438,6 +449,7 @@ class SlowARModel:
             lib().s2k_seq_free(self._seq)
             self._seq = ctypes.c_void_p()
         self._max_seq_len = 0
+        self._kv8 = None
 
     @property
     def n_past(self) -> int:
@@ -461,6 +473,19 @@ class SlowARModel:
 
     def step(self, flat_tokens: np.ndarray):
         return self._eval(flat_tokens, 1)
+
+    def eval_logprobs(self, flat_tokens: np.ndarray, n_tokens: int, n_top: int = 0):
+        """Evaluates the tokens like prefill and returns (logprob [n_tokens - 1] of each next main token, entropy
+        [n_tokens], top_ids, top_logprobs [n_tokens][n_top], None for n_top 0) (s2k_eval_logprobs)."""
+        flat = np.ascontiguousarray(flat_tokens, dtype=np.int32)
+        if flat.size != n_tokens * (self._hp.num_codebooks + 1):
+            raise S2KError(-1, f"expected {n_tokens * (self._hp.num_codebooks + 1)} ints, got {flat.size}")
+        lp, ent = np.empty(max(n_tokens - 1, 0), np.float32), np.empty(n_tokens, np.float32)
+        k = max(n_top, 0)
+        ids, top = np.empty((n_tokens, k), np.int32), np.empty((n_tokens, k), np.float32)
+        _check(lib().s2k_eval_logprobs(self._m, self._seq, _ptr(flat), n_tokens, n_top, _ptr(lp), _ptr(ent), _ptr(ids),
+                                       _ptr(top)))
+        return lp, ent, (ids if k else None), (top if k else None)
 
     def fast_decode(self, hidden: np.ndarray, prefix_codes) -> np.ndarray:
         h = np.ascontiguousarray(hidden, dtype=np.float32)
@@ -499,7 +524,11 @@ class SlowARModel:
             raise S2KError(-1, f"prompt must have {hp.num_codebooks + 1} rows")
         need = cols + max_new_tokens
         if not self._seq or self._max_seq() < need:
-            self.init_kv_cache(need)
+            kv8 = getattr(self, "_kv8", None)
+            if kv8 is not None:  # a larger cache of the same kind
+                self.init_kv8_cache(need, *kv8)
+            else:
+                self.init_kv_cache(need)
         ncb = max(hp.num_codebooks, 1)
         codes = np.zeros(ncb * max(max_new_tokens, 1), dtype=np.int32)
         nf = ctypes.c_int32(0)
