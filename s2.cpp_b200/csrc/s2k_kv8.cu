@@ -8,10 +8,10 @@
 // Each such step adds at most half of s', and a block of 16 tokens sees few
 // (the running maximum of 16 values changes about 3.4 times on average).
 //
-// The quotient is rounded exactly: the product with 1/s is within 127 * 2^-23
-// of it, so only a result that near to a half is divided again, in double
-// (where a 24-bit by 24-bit quotient that is no half stays at least 2^-33
-// away from one).  The stored integers are then a function of the inputs
+// The quotient is rounded exactly: the product with 1/s is within 127 * 2^-23 =
+// 1.5e-5 of it, so only a result that near to a half is divided again, in
+// double (where a 24-bit by 24-bit quotient that is no half stays at least
+// 2^-33 away from one).  The stored integers are then a function of the inputs
 // alone, whatever computes them.
 //
 // int8 with a block's scale rather than an 8-bit float: over a block of normal
@@ -26,16 +26,27 @@ namespace s2k {
 
 constexpr int kKv8Warps = 4;
 
-// q = round(x / s): r is the quotient to 127 * 2^-23, exact() the same in double
+// Adding 1.5 * 2^23 rounds to an integer, ties to even, and leaves it in the low mantissa bits: the conversion and
+// rounding instructions run at a quarter of an addition's rate.
+constexpr float kRound = 12582912.f;
+
+// q = round(x / s) in the low byte: r is the quotient to 1.5e-5, exact() the same in double
 template <class F>
-__device__ __forceinline__ int q8_round(float r, bool tiny, F exact) {
-    float n = rintf(r);
-    if (tiny || fabsf(fabsf(r - n) - 0.5f) < 1e-4f) n = (float)rint(exact());
-    return (int)fminf(fmaxf(n, -127.f), 127.f);
+__device__ __forceinline__ unsigned q8_round(float r, bool tiny, F exact) {
+    const float t = __fadd_rn(r, kRound);
+    unsigned q = __float_as_uint(t);
+    if (tiny || fabsf(__fsub_rn(r, __fsub_rn(t, kRound))) > 0.49998f)
+        q = (unsigned)(int)fmin(fmax(rint(exact()), -127.0), 127.0);
+    return q;
 }
 
-__device__ __forceinline__ unsigned pack4(int a, int b, int c, int d) {
-    return (unsigned)(a & 255) | (unsigned)(b & 255) << 8 | (unsigned)(c & 255) << 16 | (unsigned)(d & 255) << 24;
+// the low bytes of four words
+__device__ __forceinline__ unsigned low_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+// byte i of w as a number, exactly: 128 + q under 2^23's exponent
+__device__ __forceinline__ float byte_value(unsigned w, int i) {
+    return __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7440 + i)) - 8388736.f;
 }
 
 // One warp per (sequence, page, kv head, keys or values): lane l holds dims
@@ -85,39 +96,66 @@ __global__ void __launch_bounds__(kKv8Warps * 32) kv8_append_kernel(Kv8 c, Kv8Ro
     const bool again = lo > 0 && s != was && !zero;  // the older tokens' scale grew
     const float ratio = again ? __fdiv_rn(was, s) : 1.f;
     auto quant = [&](float y) {
-        return zero ? 0 : q8_round(__fmul_rn(y, inv), tiny, [&] { return (double)y / (double)s; });
+        return q8_round(__fmul_rn(y, inv), tiny, [&] { return zero ? 0.0 : (double)y / (double)s; });
     };
-    auto requant = [&](int q) {
-        return q8_round(__fmul_rn((float)q, ratio), tiny, [&] { return (double)q * (double)was / (double)s; });
+    auto requant = [&](unsigned w, int i) {
+        const float q = byte_value(w, i);
+        return q8_round(__fmul_rn(q, ratio), tiny, [&] { return (double)q * (double)was / (double)s; });
     };
+    if (bad) {  // x * 0 would keep a NaN
+#pragma unroll
+        for (int t = 0; t < kPage; ++t)
+#pragma unroll
+            for (int d = 0; d < D; ++d) x[t][d] = 0.f;
+    }
+    // D of a key's bytes, or 16 of a value's dimension, are words of four
     if (!is_v) {
 #pragma unroll
         for (int t = 0; t < kPage; ++t) {
-            Vec<int8_t, D> *at = reinterpret_cast<Vec<int8_t, D> *>(dst + t * HD + lane * D);
+            unsigned char *at = reinterpret_cast<unsigned char *>(dst + t * HD + lane * D);
+            unsigned w;
             if (t >= lo && t < hi) {
-                Vec<int8_t, D> u;
-#pragma unroll
-                for (int d = 0; d < D; ++d) u.v[d] = (int8_t)quant(x[t][d]);
-                *at = u;
+                w = low_bytes(quant(x[t][0]), quant(x[t][1]), D == 4 ? quant(x[t][D - 2]) : 0u, D == 4 ? quant(x[t][D - 1]) : 0u);
             } else if (t < lo && again) {
-                Vec<int8_t, D> u = *at;
-#pragma unroll
-                for (int d = 0; d < D; ++d) u.v[d] = (int8_t)requant(u.v[d]);
-                *at = u;
+                const unsigned o = D == 4 ? *reinterpret_cast<const unsigned *>(at) : *reinterpret_cast<const uint16_t *>(at);
+                w = low_bytes(requant(o, 0), requant(o, 1), D == 4 ? requant(o, 2) : 0u, D == 4 ? requant(o, 3) : 0u);
+            } else {
+                continue;
             }
+            if (D == 4) *reinterpret_cast<unsigned *>(at) = w;
+            else *reinterpret_cast<uint16_t *>(at) = (uint16_t)w;
         }
     } else {
 #pragma unroll
         for (int d = 0; d < D; ++d) {
             uint4 *at = reinterpret_cast<uint4 *>(dst + (lane * D + d) * kPage);
-            Vec<int8_t, kPage> u = {};
-            if (lo > 0 || hi < kPage) u = *reinterpret_cast<const Vec<int8_t, kPage> *>(at);
-#pragma unroll
-            for (int t = 0; t < kPage; ++t) {
-                if (t >= lo && t < hi) u.v[t] = (int8_t)quant(x[t][d]);
-                else if (t < lo && again) u.v[t] = (int8_t)requant(u.v[t]);
+            unsigned w[4] = {};
+            const bool part = lo > 0 || hi < kPage;
+            if (part) {
+                const uint4 o = *at;
+                w[0] = o.x, w[1] = o.y, w[2] = o.z, w[3] = o.w;
             }
-            *at = *reinterpret_cast<const uint4 *>(&u);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                unsigned q[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[e] = quant(x[4 * g + e][d]);
+                const unsigned fresh = low_bytes(q[0], q[1], q[2], q[3]);
+                if (!part) {
+                    w[g] = fresh;
+                    continue;
+                }
+                if (again && 4 * g < lo) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) q[e] = requant(w[g], e);
+                }
+                const unsigned older = again && 4 * g < lo ? low_bytes(q[0], q[1], q[2], q[3]) : w[g];
+                // bytes [lo, hi) are new, those before older, those behind stay
+                auto mask = [&](int n) { return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1u; };
+                const unsigned m_old = mask(lo - 4 * g), m_new = mask(hi - 4 * g) & ~m_old;
+                w[g] = (older & m_old) | (fresh & m_new) | (w[g] & ~(m_old | m_new));
+            }
+            *at = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
     if (lane == 0 && (lo == 0 || s != was)) *scale = s;
@@ -146,23 +184,27 @@ __global__ void __launch_bounds__(kKv8Warps * 32) kv8_read_kernel(Kv8 c, Kv8Rows
     const size_t blk = c.block(page, head);
     const float s = (is_v ? c.v_scale : c.k_scale)[blk];
     const int8_t *src = (is_v ? c.v : c.k) + blk * (kPage * HD);
-    Vec<int8_t, kPage> col[D];
+    // one 4-byte word (keys) or 16 bytes (values) per lane and row or dimension, all on their way at once
+    unsigned w[kPage];
     if (is_v) {
 #pragma unroll
-        for (int d = 0; d < D; ++d) col[d] = *reinterpret_cast<const Vec<int8_t, kPage> *>(src + (lane * D + d) * kPage);
+        for (int d = 0; d < D; ++d) {
+            const uint4 o = *reinterpret_cast<const uint4 *>(src + (lane * D + d) * kPage);
+            w[4 * d] = o.x, w[4 * d + 1] = o.y, w[4 * d + 2] = o.z, w[4 * d + 3] = o.w;
+        }
+    } else {
+#pragma unroll
+        for (int t = 0; t < kPage; ++t)
+            w[t] = D == 4 ? *reinterpret_cast<const unsigned *>(src + t * HD + lane * D)
+                          : *reinterpret_cast<const uint16_t *>(src + t * HD + lane * D);
     }
 #pragma unroll
     for (int t = 0; t < kPage; ++t) {
         if (t < lo || t >= hi) continue;
         float y[D];
-        if (is_v) {
 #pragma unroll
-            for (int d = 0; d < D; ++d) y[d] = __fmul_rn((float)col[d].v[t], s);
-        } else {
-            const Vec<int8_t, D> u = *reinterpret_cast<const Vec<int8_t, D> *>(src + t * HD + lane * D);
-#pragma unroll
-            for (int d = 0; d < D; ++d) y[d] = __fmul_rn((float)u.v[d], s);
-        }
+        for (int d = 0; d < D; ++d)
+            y[d] = __fmul_rn(is_v ? byte_value(w[4 * d + t / 4], t % 4) : byte_value(w[t], d), s);
         store_n<D>(y0 + (long long)(row0 + p0 + t - past) * dst.row_stride, VEC, y);
     }
 }

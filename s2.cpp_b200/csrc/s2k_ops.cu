@@ -6,6 +6,7 @@
 #include "s2k_kv8.h"
 #include "s2k_model.h"
 
+#include <atomic>
 #include <climits>
 #include <cmath>
 
@@ -19,10 +20,14 @@ namespace {
 struct OnDevice {
     int before = -1;
     s2k_status enter(int device) {
-        int n = 0;
-        if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
-            cudaGetLastError();
-            return fail(S2K_ERR_NO_DEVICE, "no CUDA device");
+        static std::atomic<int> count{0};
+        int n = count.load(std::memory_order_relaxed);
+        if (n == 0) {
+            if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
+                cudaGetLastError();
+                return fail(S2K_ERR_NO_DEVICE, "no CUDA device");
+            }
+            count.store(n, std::memory_order_relaxed);
         }
         if (device < 0 || device >= n) return fail(S2K_ERR_ARG, "device %d out of range (%d devices)", device, n);
         int cur = -1;

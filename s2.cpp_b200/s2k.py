@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from typing import Callable, Optional
 
 import numpy as np
@@ -905,7 +906,12 @@ class CodecStream:
 #
 # A decode step's operators take a few microseconds on the device, so the
 # checks here stay cheap: torch's dtype objects are compared by identity (the
-# module is looked up at the first call, the binding does not need it before).
+# module is looked up at the first call, the binding does not need it before),
+# and the C structs are packed bytes (a third of a ctypes.Structure's time).
+
+_PACK_KV8 = struct.Struct("@PPPPiiiii4x").pack    # s2k_kv8
+_PACK_ROWS = struct.Struct("@iiiiPPPP").pack      # s2k_kv8_rows
+_PACK_HEADS = struct.Struct("@Pqqi4x").pack       # s2k_heads
 
 _torch = None
 _OP_TYPES = {}  # torch dtype -> S2K_TYPE_F32 / F16 / BF16
@@ -978,8 +984,7 @@ class KV8Cache:
                 raise S2KError(-1, f"{what} is not on the CUDA device of the cache")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_pages, self.n_layers, self.n_kv_heads, self.head_dim = P, L, H, D
-        self._c = c = _KV8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), device, P, L, H, D)
-        self._ref = ctypes.byref(c)
+        self._c = _PACK_KV8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), device, P, L, H, D)
 
     @classmethod
     def empty(cls, n_pages: int, n_layers: int, n_kv_heads: int, head_dim: int, device: int = 0) -> "KV8Cache":
@@ -990,21 +995,21 @@ class KV8Cache:
                    torch.zeros(shape + (head_dim, 16), dtype=torch.int8, device=dev),
                    torch.zeros(shape, device=dev), torch.zeros(shape, device=dev))
 
-    def _rows(self, n_rows: int, past, block_table, row_start, max_rows, err) -> _KV8Rows:
-        dev, n = self.device, past.shape[0] if past.dim() == 1 else -1
-        if block_table.dim() != 2:
+    def _rows(self, n_rows: int, past, block_table, row_start, max_rows, err) -> bytes:
+        dev, shape = self.device, block_table.shape
+        if len(shape) != 2:
             raise S2KError(-1, "block_table must be [n_seqs][entries]")
-        ld = block_table.shape[1]
+        n, ld = shape
         if max_rows is None:
             if row_start is not None or n <= 0 or n_rows % n:
                 raise S2KError(-1, "max_rows is needed where rows are not shared out evenly")
             max_rows = n_rows // n
-        return _KV8Rows(n, n_rows, max_rows, ld, _ints("past", past, (n,), dev),
-                        None if row_start is None else _ints("row_start", row_start, (n + 1,), dev),
-                        _ints("block_table", block_table, (n, ld), dev),
-                        None if err is None else _ints("err", err, (1,), dev))
+        return _PACK_ROWS(n, n_rows, max_rows, ld, _ints("past", past, (n,), dev),
+                          0 if row_start is None else _ints("row_start", row_start, (n + 1,), dev),
+                          _ints("block_table", block_table, shape, dev),
+                          0 if err is None else _ints("err", err, (1,), dev))
 
-    def _heads(self, what: str, t, n_heads) -> _Heads:
+    def _heads(self, what: str, t, n_heads) -> bytes:
         shape, s = t.shape, t.stride()
         if len(s) != 3 or shape[2] != self.head_dim or (n_heads is not None and shape[1] != n_heads) or \
                 (s[2] != 1 and shape[0]):
@@ -1013,7 +1018,7 @@ class KV8Cache:
             raise S2KError(-1, f"{what} is not on CUDA device {self.device}")
         if not shape[0]:
             s = (shape[1] * shape[2], shape[2], 1)  # no rows: whatever their strides
-        return _Heads(t.data_ptr(), s[0], s[1], _op_type(what, t))
+        return _PACK_HEADS(t.data_ptr(), s[0], s[1], _op_type(what, t))
 
     def append(self, layer: int, k, v, past, block_table, row_start=None, max_rows: Optional[int] = None, err=None,
                stream=None) -> None:
@@ -1022,8 +1027,7 @@ class KV8Cache:
             raise S2KError(-1, "k and v have different shapes")
         r = self._rows(k.shape[0], past, block_table, row_start, max_rows, err)
         kh, vh = self._heads("k", k, self.n_kv_heads), self._heads("v", v, self.n_kv_heads)
-        _check(lib().s2k_kv8_append(self._ref, layer, ctypes.byref(r), ctypes.byref(kh), ctypes.byref(vh),
-                                    _op_stream(self.device, stream)))
+        _check(lib().s2k_kv8_append(self._c, layer, r, kh, vh, _op_stream(self.device, stream)))
 
     def read(self, layer: int, n_rows: int, past, block_table, row_start=None, max_rows: Optional[int] = None,
              dtype=None, out=None, err=None, stream=None):
@@ -1032,13 +1036,12 @@ class KV8Cache:
         if out is None:
             shape = (n_rows, self.n_kv_heads, self.head_dim)
             dtype = self.k_scale.dtype if dtype is None else dtype
-            out = (self.k_scale.new_empty(shape, dtype=dtype), self.k_scale.new_empty(shape, dtype=dtype))
+            out = self.k_scale.new_empty((2,) + shape, dtype=dtype).unbind(0)
         if out[0].shape[0] != n_rows or out[1].shape[0] != n_rows:
             raise S2KError(-1, f"out must hold {n_rows} rows")
         r = self._rows(n_rows, past, block_table, row_start, max_rows, err)
         kh, vh = self._heads("k", out[0], self.n_kv_heads), self._heads("v", out[1], self.n_kv_heads)
-        _check(lib().s2k_kv8_read(self._ref, layer, ctypes.byref(r), ctypes.byref(kh), ctypes.byref(vh),
-                                  _op_stream(self.device, stream)))
+        _check(lib().s2k_kv8_read(self._c, layer, r, kh, vh, _op_stream(self.device, stream)))
         return out[0], out[1]
 
     def attend(self, layer: int, q, past, block_table, row_start=None, max_rows: Optional[int] = None,
@@ -1046,16 +1049,16 @@ class KV8Cache:
         """Attention of rows q [rows][heads][head_dim] over their sequences' cached positions, causal, with the
         last `window` keys (0: all) and the first `sinks` keys visible (s2k_kv8_attend); scale defaults to
         head_dim ** -0.5.  Returns out, a tensor like q unless given."""
+        qh = self._heads("q", q, None)
         if out is None:
-            out = q.new_empty(q.shape)
-        if out.shape != q.shape:
+            out = _torch.empty_like(q)
+        elif out.shape != q.shape:
             raise S2KError(-1, "q and out have different shapes")
-        r = self._rows(q.shape[0], past, block_table, row_start, max_rows, err)
-        qh, oh = self._heads("q", q, None), self._heads("out", out, None)
-        if scale is None:
-            scale = self.head_dim ** -0.5
-        _check(lib().s2k_kv8_attend(self._ref, layer, ctypes.byref(r), ctypes.byref(qh), ctypes.byref(oh),
-                                    q.shape[1], scale, window, sinks, _op_stream(self.device, stream)))
+        shape = q.shape
+        r = self._rows(shape[0], past, block_table, row_start, max_rows, err)
+        _check(lib().s2k_kv8_attend(self._c, layer, r, qh, self._heads("out", out, None), shape[1],
+                                    self.head_dim ** -0.5 if scale is None else scale, window, sinks,
+                                    _op_stream(self.device, stream)))
         return out
 
 

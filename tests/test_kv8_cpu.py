@@ -110,6 +110,10 @@ def test_structs_match_header():
         names = [n.strip().lstrip("*") for d in body.split(";") if d.strip() for n in d.strip().split(None, 1)[1].split(",")]
         names = [n.split()[-1].lstrip("*") for n in names]
         assert names == [f for f, _ in cls._fields_]
+    # the packed forms that the binding passes
+    for pack, s in ((s2k._PACK_KV8, cache(device=3)), (s2k._PACK_ROWS, rows(row_start=A + 64, err=A + 128)),
+                    (s2k._PACK_HEADS, heads(type=30))):
+        assert pack(*[getattr(s, f) or 0 for f, _ in s._fields_]) == bytes(s)
 
 
 def test_plain_append_by_steps_stays_near_one_call():
