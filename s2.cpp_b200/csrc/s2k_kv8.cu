@@ -30,13 +30,16 @@ constexpr int kKv8Warps = 4;
 // rounding instructions run at a quarter of an addition's rate.
 constexpr float kRound = 12582912.f;
 
-// q = round(x / s) in the low byte: r is the quotient to 1.5e-5, exact() the same in double
-template <class F>
-__device__ __forceinline__ unsigned q8_round(float r, bool tiny, F exact) {
+// round(a * b / s), b = 1 or an older scale; kept out of line: 64 divisions in double in the loop's code made the
+// instruction cache the bound (124 us for eight prompts).
+__device__ __noinline__ unsigned q8_exact(float a, float b, float s) {
+    return s == 0.f ? 0u : (unsigned)(int)fmin(fmax(rint((double)a * (double)b / (double)s), -127.0), 127.0);
+}
+// q = round(a * b / s) in the low byte; r is the quotient to 1.5e-5
+__device__ __forceinline__ unsigned q8_round(float r, bool tiny, float a, float b, float s) {
     const float t = __fadd_rn(r, kRound);
     unsigned q = __float_as_uint(t);
-    if (tiny || fabsf(__fsub_rn(r, __fsub_rn(t, kRound))) > 0.49998f)
-        q = (unsigned)(int)fmin(fmax(rint(exact()), -127.0), 127.0);
+    if (tiny || fabsf(__fsub_rn(r, __fsub_rn(t, kRound))) > 0.49998f) q = q8_exact(a, b, s);
     return q;
 }
 
@@ -68,19 +71,19 @@ __global__ void __launch_bounds__(kKv8Warps * 32) kv8_append_kernel(Kv8 c, Kv8Ro
     const int pg = past / kPage + pi, p0 = pg * kPage;
     if (p0 >= past + n) return;
     const int lo = max(past - p0, 0), hi = min(past + n - p0, kPage);  // slots [lo, hi) are new, [0, lo) older
-    const int page = kv8_page(c, r, b, pg);
-    if (page < 0) return;
     const Rows &src = is_v ? v : k;
     const T *x0 = reinterpret_cast<const T *>(src.p) + (long long)head * src.head_stride + lane * D;
-    const size_t blk = c.block(page, head);
-    float *scale = (is_v ? c.v_scale : c.k_scale) + blk;
-    int8_t *dst = (is_v ? c.v : c.k) + blk * (kPage * HD);
     float x[kPage][D];
     unsigned top = 0;  // |x| as integers: NaN and infinity order above every finite value
     // slots without a new token load a neighbour's: a condition around a load would be waited for
 #pragma unroll
     for (int t = 0; t < kPage; ++t)
         load_n<D>(x0 + (long long)(row0 + p0 + min(max(t, lo), hi - 1) - past) * src.row_stride, VEC, x[t]);
+    const int page = kv8_page(c, r, b, pg);
+    if (page < 0) return;
+    const size_t blk = c.block(page, head);
+    float *scale = (is_v ? c.v_scale : c.k_scale) + blk;
+    int8_t *dst = (is_v ? c.v : c.k) + blk * (kPage * HD);
 #pragma unroll
     for (int t = 0; t < kPage; ++t)
 #pragma unroll
@@ -95,12 +98,10 @@ __global__ void __launch_bounds__(kKv8Warps * 32) kv8_append_kernel(Kv8 c, Kv8Ro
     const float inv = zero ? 0.f : __fdiv_rn(1.f, s);
     const bool again = lo > 0 && s != was && !zero;  // the older tokens' scale grew
     const float ratio = again ? __fdiv_rn(was, s) : 1.f;
-    auto quant = [&](float y) {
-        return q8_round(__fmul_rn(y, inv), tiny, [&] { return zero ? 0.0 : (double)y / (double)s; });
-    };
+    auto quant = [&](float y) { return q8_round(__fmul_rn(y, inv), tiny, y, 1.f, zero ? 0.f : s); };
     auto requant = [&](unsigned w, int i) {
         const float q = byte_value(w, i);
-        return q8_round(__fmul_rn(q, ratio), tiny, [&] { return (double)q * (double)was / (double)s; });
+        return q8_round(__fmul_rn(q, ratio), tiny, q, was, s);
     };
     if (bad) {  // x * 0 would keep a NaN
 #pragma unroll
