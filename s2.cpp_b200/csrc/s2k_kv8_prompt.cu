@@ -427,6 +427,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
         // positions of the warp's rows
         const int s_lo = slot0 + min(ls - lane, nslots - 1), s_hi = slot0 + min(ls - lane + 31, nslots - 1);
         const int p_min = past + row_of(s_lo), p_max = past + row_of(s_hi);
+        const int wlo_row = a.window ? max(pos - a.window + 1, 0) : 0;  // the first position in the row's window
         const float smul = wide ? sm.qmul[row] : a.scale * 1.44269504f;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t S = tmem + lanes + w * kPM, O = tmem + lanes + 2 * kPM + w * kPM;
@@ -481,48 +482,57 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 hi = max(hi, m.p0[i]);
                 vmax = fmaxf(vmax, m.vs[i]);
             }
-            const bool edge = hi + kPage - 1 > p_min || (a.window && lo <= p_max - a.window && hi + kPage > a.sinks) ||
-                              a.scale < 0.f;  // the largest product is not the largest score's
+            const bool edge = hi + kPage - 1 > p_min || (a.window && lo <= p_max - a.window && hi + kPage > a.sinks) || a.scale < 0.f;
             // bit i: the row sees token i of page pg
-            auto below = [](long long n) { return n <= 0 ? 0u : n >= kPage ? 0xffffu : (1u << (int)n) - 1u; };
+            auto below = [](int n) { return 0xffffu >> (kPage - min(max(n, 0), kPage)); };
             auto seen = [&](int pg) {
-                const long long p0 = m.p0[pg];
-                uint32_t bits = below(pos + 1 - p0);
-                if (a.window) bits &= ~below(pos + 1ll - a.window - p0) | below(a.sinks - p0);
-                return bits;
+                const int p0 = m.p0[pg];
+                return below(pos + 1 - p0) & (~below(wlo_row - p0) | below(a.sinks - p0));
             };
             // the step's largest score.  Loops stay rolled: unrolled, with the next columns' loads ahead, they took twice
             // as long (the instruction cache serves ten warps in five places).
             float mx = -INFINITY;
-            uint32_t any = !edge;
+            uint32_t any = 0;
+            auto whole_max = [&](const int(&y)[32], float k0, float k1) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < kPage; i += 4) {
+                        t0 = fmaxf(fmaxf(t0, __int_as_float(y[16 * e + i])), __int_as_float(y[16 * e + i + 1]));
+                        t1 = fmaxf(fmaxf(t1, __int_as_float(y[16 * e + i + 2])), __int_as_float(y[16 * e + i + 3]));
+                    }
+                    mx = fmaxf(mx, fmaxf(t0, t1) * (e ? k1 : k0));
+                }
+            };
             if (!edge) {
 #pragma unroll 1
                 for (int ch = 0; ch < 4; ++ch) {
                     int y[32];
                     tmem_ld32(S + 32 * ch, y);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-                        for (int i = 0; i < kPage; i += 4) {
-                            t0 = fmaxf(fmaxf(t0, __int_as_float(y[16 * e + i])), __int_as_float(y[16 * e + i + 1]));
-                            t1 = fmaxf(fmaxf(t1, __int_as_float(y[16 * e + i + 2])), __int_as_float(y[16 * e + i + 3]));
-                        }
-                        mx = fmaxf(mx, fmaxf(t0, t1) * (m.ks[2 * ch + e] * smul));
-                    }
+                    whole_max(y, m.ks[2 * ch] * smul, m.ks[2 * ch + 1] * smul);
                 }
+                any = 1;
             } else {
                 vmax = 0.f;
 #pragma unroll 1
-                for (int pg = 0; pg < kPPages; ++pg) {
-                    int y[16];
-                    tmem_ld16(S + 16 * pg, y);
-                    const uint32_t bits = seen(pg);
-                    const float ks = m.ks[pg] * smul;
-                    if (bits) vmax = fmaxf(vmax, m.vs[pg]);
-#pragma unroll
-                    for (int i = 0; i < kPage; ++i) mx = fmaxf(mx, bits >> i & 1 ? __int_as_float(y[i]) * ks : -INFINITY);
+                for (int ch = 0; ch < 4; ++ch) {
+                    int y[32];
+                    tmem_ld32(S + 32 * ch, y);
+                    const float k0 = m.ks[2 * ch] * smul, k1 = m.ks[2 * ch + 1] * smul;
+                    const uint32_t b0 = seen(2 * ch), b1 = seen(2 * ch + 1), bits = b0 | b1 << 16;
                     any |= bits;
+                    if (b0) vmax = fmaxf(vmax, m.vs[2 * ch]);
+                    if (b1) vmax = fmaxf(vmax, m.vs[2 * ch + 1]);
+                    if (__all_sync(kAll, bits == 0)) continue;
+                    // the largest product is the largest score's unless the scale is negative
+                    if (__all_sync(kAll, bits == ~0u) && a.scale >= 0.f) {
+                        whole_max(y, k0, k1);
+                        continue;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        mx = fmaxf(mx, bits >> i & 1 ? __int_as_float(y[i]) * (i < 16 ? k0 : k1) : -INFINITY);
                 }
             }
             // keys in view and no number among their scores: an infinite or NaN query or scale
@@ -591,17 +601,31 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 tc_fence_before();
                 mbar_arrive(&sm.pfull[w][h]);
             };
-            auto all_weights = [&](auto masked) {
+            if (!edge) {
 #pragma unroll 1
                 for (int ch = 0; ch < 4; ++ch) {
                     int y[32];
                     tmem_ld32(S + 32 * ch, y);
-                    weights(ch, y, masked);
+                    weights(ch, y, std::false_type());
                     if (ch & 1) half_done(ch / 2);
                 }
-            };
-            if (edge) all_weights(std::true_type());
-            else all_weights(std::false_type());
+            } else {
+#pragma unroll 1
+                for (int ch = 0; ch < 4; ++ch) {
+                    const uint32_t bits = seen(2 * ch) | seen(2 * ch + 1) << 16;
+                    if (__all_sync(kAll, bits == 0)) {  // nothing of it in the warp's view
+                        const uint32_t none[16] = {};
+                        tmem_st16(S + 32 * ch, none);
+                        if (wide) tmem_st16(S + 32 * ch + 16, none);
+                    } else {
+                        int y[32];
+                        tmem_ld32(S + 32 * ch, y);
+                        if (__all_sync(kAll, bits == ~0u)) weights(ch, y, std::false_type());
+                        else weights(ch, y, std::true_type());
+                    }
+                    if (ch & 1) half_done(ch / 2);
+                }
+            }
             if (wide) {
                 sm.stat[t % kPMeta][row] = make_float4(ref, l0 + l1, vref * (1.f / kPStepTop), 0.f);
                 mbar_arrive(&sm.tfull[t % kPMeta]);
