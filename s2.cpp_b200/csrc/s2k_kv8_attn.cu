@@ -115,7 +115,7 @@ struct DecodeSmem {
     float qmul[SLOTS];
     float m[kDWarps][SLOTS], l[kDWarps][SLOTS];
     // what the cluster's CTAs send: their outputs for this CTA's share, and (maximum, sum)
-    float4 from[SLOTS * HD / 4];
+    float4 from[SLOTS * HD / 4 + kMaxCluster];
     float2 ml[kMaxCluster][SLOTS];
 };
 
@@ -129,7 +129,7 @@ __device__ __forceinline__ int key_at(int x) {
 
 template <int HD, int TYPE>
 __global__ void __launch_bounds__(kDThreads, 3)
-    kv8_decode_kernel(Kv8 c, Kv8Rows r, Kv8Attn a, int cs_log2, float inv_group, int vec) {
+    kv8_decode_kernel(Kv8 c, Kv8Rows r, Kv8Attn a, int cs, float inv_group, int vec) {
     using T = typename OType<TYPE>::T;
     using Dg = Digits<TYPE>;
     constexpr int SLOTS = Dg::slots, STAGES = kDStages<HD>;
@@ -139,8 +139,8 @@ __global__ void __launch_bounds__(kDThreads, 3)
     extern __shared__ uint8_t raw[];
     auto &sm = *reinterpret_cast<DecodeSmem<HD, SLOTS> *>((reinterpret_cast<uintptr_t>(raw) + 127) & ~uintptr_t(127));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, li = lane >> 2, lc = lane & 3;
-    const int cs = 1 << cs_log2, rank = blockIdx.x & (cs - 1);  // clusters lie along x
-    const int b = blockIdx.x >> cs_log2, kvh = blockIdx.y, tile = blockIdx.z;
+    const int b = blockIdx.x / cs, rank = blockIdx.x - b * cs;  // clusters lie along x
+    const int kvh = blockIdx.y, tile = blockIdx.z;
     const int G = a.n_heads / c.n_kv_heads;
     int row0, n, past;
     // the same for every CTA of the cluster: none is left waiting
@@ -161,7 +161,8 @@ __global__ void __launch_bounds__(kDThreads, 3)
     const int total = ns + pos_hi / kPage - fw + 1;
     // this CTA's pages, in pairs; pair k of the warp is pages 2 * (warp + k * kDWarps) and the next
     const int pairs = (total + 1) / 2;
-    const int first = pairs * rank >> cs_log2, last = pairs * (rank + 1) >> cs_log2;
+    const int each = pairs / cs, more = pairs - each * cs;  // the first `more` CTAs have one more
+    const int first = each * rank + min(rank, more), last = first + each + (rank < more);
     const int mine = last - first > warp ? (last - first - warp + kDWarps - 1) / kDWarps : 0;
     if (cs > 1) cluster_arrive();  // this CTA runs: others may store into its shared memory
     // lanes 2k and 2k + 1 hold pair k of the warp's current 16 pairs, and of the next 16: the physical page, or -1,
@@ -385,7 +386,7 @@ __global__ void __launch_bounds__(kDThreads, 3)
     }
     __syncthreads();
     constexpr int kItems = SLOTS * HD / 4;  // of 4 dims; with a cluster each CTA joins a share of them
-    const int share = kItems >> cs_log2;
+    const int share = (kItems + cs - 1) / cs;
     auto put = [&](int item, float sum, float4 v) {
         const int st = tile * SLOTS + item / (HD / 4);
         if (item / (HD / 4) >= nslots) return;
@@ -408,7 +409,10 @@ __global__ void __launch_bounds__(kDThreads, 3)
             sum += sm.l[w][sl];
         }
         if (cs == 1) put(item, sum, v);
-        else st_cluster(in_cta(&sm.from[rank * share + item % share], item / share), v);
+        else {
+            const int owner = item / share;
+            st_cluster(in_cta(&sm.from[rank * share + item - owner * share], owner), v);
+        }
     }
     if (cs == 1) return;
     for (int x = tid; x < SLOTS * cs; x += kDThreads) {
@@ -420,7 +424,7 @@ __global__ void __launch_bounds__(kDThreads, 3)
     }
     cluster_arrive();
     cluster_wait();  // from here no CTA reaches into another's shared memory
-    for (int x = tid; x < share; x += kDThreads) {
+    for (int x = tid; x < min(share, kItems - rank * share); x += kDThreads) {
         const int item = rank * share + x, sl = item / (HD / 4);
         float mm = -INFINITY, sum = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -458,22 +462,22 @@ static cudaError_t decode_setup() {
 }
 
 template <int HD, int TYPE>
-static cudaError_t decode_launch(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, int cs_log2, int tiles,
+static cudaError_t decode_launch(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, int cs, int tiles,
                                  cudaStream_t st) {
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1u << cs_log2;
+    attr[0].val.clusterDim.x = cs;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)r.n_seqs << cs_log2, c.n_kv_heads, tiles);
+    cfg.gridDim = dim3((unsigned)r.n_seqs * cs, c.n_kv_heads, tiles);
     cfg.blockDim = dim3(kDThreads);
     cfg.dynamicSmemBytes = decode_smem<HD, TYPE>();
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = cs_log2 > 0 ? 1 : 0;
+    cfg.numAttrs = cs > 1 ? 1 : 0;
     const float inv_group = 1.0f / (float)(a.n_heads / c.n_kv_heads);
     const int vec = rows_vec(a.q, 4) && rows_vec(a.out, 4);
-    return cudaLaunchKernelEx(&cfg, kv8_decode_kernel<HD, TYPE>, c, r, a, cs_log2, inv_group, vec);
+    return cudaLaunchKernelEx(&cfg, kv8_decode_kernel<HD, TYPE>, c, r, a, cs, inv_group, vec);
 }
 
 cudaError_t launch_kv8_attend(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, cudaStream_t st) {
@@ -501,13 +505,15 @@ cudaError_t launch_kv8_attend(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, 
     // pages of one unit at most
     long long pages = r.table_ld;
     if (a.window) pages = std::min(pages, ((long long)a.window + r.max_rows + a.sinks) / kPage + 3);
-    // CTAs per unit.  A CTA's start and its join cost about as much as 40 pages, so pieces of 48 to 96 pages are
-    // best where the machine is full (64 sequences of up to 2523 tokens: 45.6 us whole, 42.9 halved, 51 in
-    // quarters; 8 of up to 6095: 28.7 halved, 20.5 quartered, 23.3 in eighths); with SMs left over, down to one
-    // pair of pages per warp (one sequence of 512 tokens: 6.7 us in the kernel whole, 5.1 in pieces).
-    int cs = 0;
-    while (cs < 4 && (pages > 96LL << cs || (units << (cs + 1) <= d.sms && pages > 8LL << cs))) ++cs;
-    if ((long long)r.n_seqs << cs > 0x7fffffffLL) return cudaErrorInvalidValue;
+    // CTAs per unit.  A CTA's start and its join cost about as much as 40 pages: pieces of about 64 pages are best
+    // where the machine is full (64 sequences of up to 2523 tokens: 46 us whole, 43.6 halved, 48 in thirds; 8 of up
+    // to 6095: 20.6 in fourths, 18.9 in sixths, 24.2 in sevenths; 16 of 4000 visible ones: 18.4 in thirds, 16.4 in
+    // fourths, 22.5 in sixths).  With SMs left over, down to a pair of pages per warp (one sequence of 512 tokens:
+    // 6.7 us in the kernel whole, 5.1 in pieces).
+    long long want = (pages + 32) / 64;
+    if (units * want < d.sms) want = std::min(d.sms / units, pages / (2 * kDWarps));
+    const int cs = (int)std::min<long long>(std::max<long long>(want, 1), kMaxCluster);
+    if ((long long)r.n_seqs * cs > 0x7fffffffLL) return cudaErrorInvalidValue;
     count_launch();
     return kv8_dispatch(c.head_dim, a.q.type, [&](auto hd, auto type) {
         return decode_launch<hd, type>(c, r, a, cs, tiles, st);
