@@ -76,6 +76,18 @@ struct alignas(16) LpSums {
     }
 };
 
+// Joins the lanes' sums, groups of `width` lanes (a power of two) each.
+__device__ void lp_join_lanes(LpSums &s, int width) {
+    for (int o = width >> 1; o > 0; o >>= 1) {
+        LpSums q;
+        q.m = __shfl_xor_sync(0xffffffffu, s.m, o);
+        q.c = __shfl_xor_sync(0xffffffffu, s.c, o);
+        q.d = __shfl_xor_sync(0xffffffffu, s.d, o);
+        q.t = __shfl_xor_sync(0xffffffffu, s.t, o);
+        s.join(q);
+    }
+}
+
 struct LpSmem {
     LpSums warp[kLpThreads / 32];
     LpSums row[kMaxCluster];             // the cluster's CTAs, in its first
@@ -304,26 +316,17 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(LogprobArgs a, 
     }
 
     // join the threads, the warps, then the cluster's CTAs
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        LpSums q;
-        q.m = __shfl_xor_sync(0xffffffffu, s.m, o);
-        q.c = __shfl_xor_sync(0xffffffffu, s.c, o);
-        q.d = __shfl_xor_sync(0xffffffffu, s.d, o);
-        q.t = __shfl_xor_sync(0xffffffffu, s.t, o);
-        s.join(q);
-    }
+    lp_join_lanes(s, 32);
     if (lane == 0) sm.warp[warp] = s;
     __syncthreads();
     if (k) lp_select(sm.cand, min(sm.count, kLpCap), k, sm.best);
     if (cs > 1) cluster_wait();
-    if (tid == 0) {
-        for (int w = 1; w < kLpThreads / 32; ++w) s.join(sm.warp[w]);
-        if (cs > 1) {
-            const uint32_t at = in_cta(&sm.row[rank], 0);
-            st_cluster(at, make_float4(s.m, s.c, s.d, s.t));
-        } else {
-            sm.row[0] = s;
+    if (warp == 0) {
+        s = sm.warp[lane % (kLpThreads / 32)];
+        lp_join_lanes(s, kLpThreads / 32);
+        if (lane == 0) {
+            if (cs > 1) st_cluster(in_cta(&sm.row[rank], 0), make_float4(s.m, s.c, s.d, s.t));
+            else sm.row[0] = s;
         }
     }
     if (cs > 1) {
@@ -334,16 +337,33 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(LogprobArgs a, 
         cluster_arrive();
         cluster_wait();
         if (rank) return;
+        if (warp == 0) {
+            s = lane < cs ? sm.row[lane] : LpSums();
+            lp_join_lanes(s, kMaxCluster);
+            // k keys of one CTA reach its last one: smaller ones are none of the row's
+            lp_key_t last = k && lane < cs ? sm.top[lane][k - 1] : 0;
+#pragma unroll
+            for (int o = kMaxCluster / 2; o > 0; o >>= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+            __syncwarp();
+            if (lane == 0) {
+                sm.row[0] = s;
+                sm.tau = last;
+                sm.count = 0;
+            }
+        }
+        __syncthreads();
         if (k) {
-            for (int i = tid; i < cs * k; i += kLpThreads) sm.cand[i] = sm.top[i / k][i % k];
+            for (int i = tid; i < cs * k; i += kLpThreads) {
+                const lp_key_t key = sm.top[i / k][i % k];
+                if (key && key >= sm.tau) sm.cand[atomicAdd(&sm.count, 1)] = key;
+            }
             __syncthreads();
-            lp_select(sm.cand, cs * k, k, sm.best);
+            lp_select(sm.cand, sm.count, k, sm.best);
         }
     } else {
         __syncthreads();
     }
     s = sm.row[0];
-    for (int r = 1; r < cs; ++r) s.join(sm.row[r]);
     if (s.m == INFINITY) s.d = NAN;
     const bool none = s.m == -INFINITY && s.d == 0.f;  // every token masked (a NaN reaches d)
     const float M = s.m == -INFINITY ? 0.f : s.m;
