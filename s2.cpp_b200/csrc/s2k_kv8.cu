@@ -35,12 +35,17 @@ constexpr float kRound = 12582912.f;
 __device__ __noinline__ unsigned q8_exact(float a, float b, float s) {
     return s == 0.f ? 0u : (unsigned)(int)fmin(fmax(rint((double)a * (double)b / (double)s), -127.0), 127.0);
 }
-// q = round(a * b / s) in the low byte; r is the quotient to 1.5e-5
-__device__ __forceinline__ unsigned q8_round(float r, bool tiny, float a, float b, float s) {
+// q = round(r) in the low byte; far: the largest distance of an r from its integer so far
+__device__ __forceinline__ unsigned q8_fast(float r, float &far) {
     const float t = __fadd_rn(r, kRound);
-    unsigned q = __float_as_uint(t);
-    if (tiny || fabsf(__fsub_rn(r, __fsub_rn(t, kRound))) > 0.49998f) q = q8_exact(a, b, s);
-    return q;
+    far = fmaxf(far, fabsf(__fsub_rn(r, __fsub_rn(t, kRound))));
+    return __float_as_uint(t);
+}
+// q = round(a * b / s) in the low byte; r is the quotient to 1.5e-5
+__device__ __forceinline__ unsigned q8_careful(float r, bool tiny, float a, float b, float s) {
+    float far = 0.f;
+    const unsigned q = q8_fast(r, far);
+    return tiny || far > 0.49998f ? q8_exact(a, b, s) : q;
 }
 
 // the low bytes of four words
@@ -98,67 +103,78 @@ __global__ void __launch_bounds__(kKv8Warps * 32) kv8_append_kernel(Kv8 c, Kv8Ro
     const float inv = zero ? 0.f : __fdiv_rn(1.f, s);
     const bool again = lo > 0 && s != was && !zero;  // the older tokens' scale grew
     const float ratio = again ? __fdiv_rn(was, s) : 1.f;
-    auto quant = [&](float y) { return q8_round(__fmul_rn(y, inv), tiny, y, 1.f, zero ? 0.f : s); };
-    auto requant = [&](unsigned w, int i) {
-        const float q = byte_value(w, i);
-        return q8_round(__fmul_rn(q, ratio), tiny, q, was, s);
-    };
     if (bad) {  // x * 0 would keep a NaN
 #pragma unroll
         for (int t = 0; t < kPage; ++t)
 #pragma unroll
             for (int d = 0; d < D; ++d) x[t][d] = 0.f;
     }
-    // D of a key's bytes, or 16 of a value's dimension, are words of four
-    if (!is_v) {
+    // D of a key's bytes, or 16 of a value's dimension, are words of four.  The first pass rounds without a branch; a
+    // lane that was too near to a half somewhere (one in 400) goes over its values again, as does every lane where older
+    // tokens are rounded again.
+    float far = 0.f;
+    auto pass = [&](auto careful) {
+        auto quant = [&](float y) {
+            const float r = __fmul_rn(y, inv);
+            return careful ? q8_careful(r, tiny, y, 1.f, zero ? 0.f : s) : q8_fast(r, far);
+        };
+        auto requant = [&](unsigned w, int i) {
+            const float q = byte_value(w, i);
+            return q8_careful(__fmul_rn(q, ratio), tiny, q, was, s);
+        };
+        const bool older_too = careful && again;
+        if (!is_v) {
 #pragma unroll
-        for (int t = 0; t < kPage; ++t) {
-            unsigned char *at = reinterpret_cast<unsigned char *>(dst + t * HD + lane * D);
-            unsigned w;
-            if (t >= lo && t < hi) {
-                w = low_bytes(quant(x[t][0]), quant(x[t][1]), D == 4 ? quant(x[t][D - 2]) : 0u, D == 4 ? quant(x[t][D - 1]) : 0u);
-            } else if (t < lo && again) {
-                const unsigned o = D == 4 ? *reinterpret_cast<const unsigned *>(at) : *reinterpret_cast<const uint16_t *>(at);
-                w = low_bytes(requant(o, 0), requant(o, 1), D == 4 ? requant(o, 2) : 0u, D == 4 ? requant(o, 3) : 0u);
-            } else {
-                continue;
-            }
-            if (D == 4) *reinterpret_cast<unsigned *>(at) = w;
-            else *reinterpret_cast<uint16_t *>(at) = (uint16_t)w;
-        }
-    } else {
-#pragma unroll
-        for (int d = 0; d < D; ++d) {
-            uint4 *at = reinterpret_cast<uint4 *>(dst + (lane * D + d) * kPage);
-            unsigned w[4] = {};
-            const bool part = lo > 0 || hi < kPage;
-            if (part) {
-                const uint4 o = *at;
-                w[0] = o.x, w[1] = o.y, w[2] = o.z, w[3] = o.w;
-            }
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                unsigned q[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) q[e] = quant(x[4 * g + e][d]);
-                const unsigned fresh = low_bytes(q[0], q[1], q[2], q[3]);
-                if (!part) {
-                    w[g] = fresh;
+            for (int t = 0; t < kPage; ++t) {
+                unsigned char *at = reinterpret_cast<unsigned char *>(dst + t * HD + lane * D);
+                unsigned w;
+                if (t >= lo && t < hi) {
+                    w = low_bytes(quant(x[t][0]), quant(x[t][1]), D == 4 ? quant(x[t][D - 2]) : 0u, D == 4 ? quant(x[t][D - 1]) : 0u);
+                } else if (t < lo && older_too) {
+                    const unsigned o = D == 4 ? *reinterpret_cast<const unsigned *>(at) : *reinterpret_cast<const uint16_t *>(at);
+                    w = low_bytes(requant(o, 0), requant(o, 1), D == 4 ? requant(o, 2) : 0u, D == 4 ? requant(o, 3) : 0u);
+                } else {
                     continue;
                 }
-                if (again && 4 * g < lo) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) q[e] = requant(w[g], e);
-                }
-                const unsigned older = again && 4 * g < lo ? low_bytes(q[0], q[1], q[2], q[3]) : w[g];
-                // bytes [lo, hi) are new, those before older, those behind stay
-                auto mask = [&](int n) { return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1u; };
-                const unsigned m_old = mask(lo - 4 * g), m_new = mask(hi - 4 * g) & ~m_old;
-                w[g] = (older & m_old) | (fresh & m_new) | (w[g] & ~(m_old | m_new));
+                if (D == 4) *reinterpret_cast<unsigned *>(at) = w;
+                else *reinterpret_cast<uint16_t *>(at) = (uint16_t)w;
             }
-            *at = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                uint4 *at = reinterpret_cast<uint4 *>(dst + (lane * D + d) * kPage);
+                unsigned w[4] = {};
+                const bool part = lo > 0 || hi < kPage;
+                if (part) {
+                    const uint4 o = *at;
+                    w[0] = o.x, w[1] = o.y, w[2] = o.z, w[3] = o.w;
+                }
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    unsigned q[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) q[e] = quant(x[4 * g + e][d]);
+                    const unsigned fresh = low_bytes(q[0], q[1], q[2], q[3]);
+                    if (!part) {
+                        w[g] = fresh;
+                        continue;
+                    }
+                    if (older_too && 4 * g < lo) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) q[e] = requant(w[g], e);
+                    }
+                    const unsigned older = older_too && 4 * g < lo ? low_bytes(q[0], q[1], q[2], q[3]) : w[g];
+                    // bytes [lo, hi) are new, those before older, those behind stay
+                    auto mask = [&](int n) { return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1u; };
+                    const unsigned m_old = mask(lo - 4 * g), m_new = mask(hi - 4 * g) & ~m_old;
+                    w[g] = (older & m_old) | (fresh & m_new) | (w[g] & ~(m_old | m_new));
+                }
+                *at = make_uint4(w[0], w[1], w[2], w[3]);
+            }
         }
-    }
+    };
+    if (!tiny && !again) pass(std::false_type());
+    if (tiny || again || far > 0.49998f) pass(std::true_type());
     if (lane == 0 && (lo == 0 || s != was)) *scale = s;
 }
 
