@@ -2023,10 +2023,11 @@ S2K_API s2k_status s2k_seq_load_kv(s2k_seq *s, const uint16_t *k, const uint16_t
     if (s->is_kv8() && n_pos > 0) {
         // rounded into the 8-bit blocks layer by layer, as one call of n_pos tokens stores them
         CU(cudaStreamSynchronize(m->stream));
-        CU(cudaMemsetAsync(&s->dev->state, 0, sizeof(SeqState), m->stream));
         __half *rows = nullptr;
         CU(m->alloc(&rows, 2 * (size_t)n_pos * kvs));
-        cudaError_t e = cudaSuccess;
+        // from here the positions held are overwritten: the sequence is empty until all are stored
+        s->n_past = 0;
+        cudaError_t e = cudaMemsetAsync(&s->dev->state, 0, sizeof(SeqState), m->stream);
         for (int l = 0; l < L && e == cudaSuccess; ++l) {
             const size_t n = (size_t)n_pos * kvs, at = (size_t)l * n;
             if ((e = cudaMemcpyAsync(rows, k + at, n * 2, cudaMemcpyHostToDevice, m->stream))) break;

@@ -198,3 +198,25 @@ def test_refusals(small_gpu, small_model_data):
         with pytest.raises(s2k.S2KError) as e:
             m.eval_logprobs(p.T.reshape(-1).copy(), 4, n_top=n_top)
         assert e.value.status == ARG
+
+
+def test_a_failed_restore_leaves_the_sequence_as_it_was(small_gpu, small_model_data):
+    """No memory for the rows: the device's position must not part from the host's."""
+    hp, _ = small_model_data
+    m = small_gpu
+    p = synthetic.text_prompt(hp, 4, seed=9).T.copy()
+    shape = (hp.block_count, 20, hp.head_count_kv, hp.head_dim)
+    k = np.ones(shape, np.float16)
+    got = []
+    for fail in (False, True):
+        m.init_kv8_cache(64)
+        m.prefill(p[:3].reshape(-1).copy(), 3)
+        if fail:
+            m.fail_alloc(0)
+            with pytest.raises(s2k.S2KError):
+                m.load_kv(k, k)
+            m.fail_alloc(-1)
+        assert m.n_past == 3
+        got.append(m.step(p[3]))
+    for a, b in zip(*got):
+        assert np.array_equal(a, b)
