@@ -13,6 +13,7 @@ on a machine without it raises, there is no fallback path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import struct
@@ -940,6 +941,16 @@ def _op_stream(device: int, stream) -> int:
     return _raw_stream(device) if stream is None else int(getattr(stream, "cuda_stream", stream))
 
 
+def _new_on(stream, device: int):
+    """Context in which new tensors belong to `stream` (None: the current one): the allocator may otherwise hand out
+    memory that the current stream still uses."""
+    if stream is None:
+        return contextlib.nullcontext()
+    if not hasattr(stream, "cuda_stream"):
+        stream = _torch.cuda.ExternalStream(int(stream), device=device) if stream else _torch.cuda.default_stream(device)
+    return _torch.cuda.stream(stream)
+
+
 def _ints(what: str, t, shape, device: int) -> int:
     """Data pointer of a contiguous int32 tensor of `device`."""
     if t.dtype is not _torch.int32 or t.shape != shape or not t.is_contiguous():
@@ -959,7 +970,8 @@ class KV8Cache:
       k_scale, v_scale   float32 [pages][layers][kv_heads]
 
     `append`, `read` and `attend` enqueue on the current torch stream of the
-    cache's device (or `stream`) and do not wait.  Their rows belong to
+    cache's device (or `stream`, which results that are not given then belong
+    to) and do not wait.  Their rows belong to
     sequences: past [n_seqs] positions held before the call, block_table
     [n_seqs][entries] page numbers, row_start [n_seqs + 1] first row of each
     sequence (None: the rows are shared out evenly), max_rows the most rows of
@@ -1036,7 +1048,8 @@ class KV8Cache:
         if out is None:
             shape = (n_rows, self.n_kv_heads, self.head_dim)
             dtype = self.k_scale.dtype if dtype is None else dtype
-            out = self.k_scale.new_empty((2,) + shape, dtype=dtype).unbind(0)
+            with _new_on(stream, self.device):
+                out = self.k_scale.new_empty((2,) + shape, dtype=dtype).unbind(0)
         if out[0].shape[0] != n_rows or out[1].shape[0] != n_rows:
             raise S2KError(-1, f"out must hold {n_rows} rows")
         r = self._rows(n_rows, past, block_table, row_start, max_rows, err)
@@ -1051,7 +1064,11 @@ class KV8Cache:
         head_dim ** -0.5.  Returns out, a tensor like q unless given."""
         qh = self._heads("q", q, None)
         if out is None:
-            out = _torch.empty_like(q)
+            if stream is None:
+                out = _torch.empty_like(q)
+            else:
+                with _new_on(stream, self.device):
+                    out = _torch.empty_like(q)
         elif out.shape != q.shape:
             raise S2KError(-1, "q and out have different shapes")
         shape = q.shape
@@ -1074,12 +1091,13 @@ def logprobs(logits, targets=None, n_top: int = 0, stream=None):
     if dev < 0:
         raise S2KError(-1, "logits is not on a CUDA device")
     tgt = None if targets is None else _ints("targets", targets, (rows,), dev)
-    logprob = None if targets is None else logits.new_empty(rows, dtype=T.float32)
-    entropy = logits.new_empty(rows, dtype=T.float32)
     ids = top = None
-    if n_top > 0:
-        ids = logits.new_empty((rows, n_top), dtype=T.int32)
-        top = logits.new_empty((rows, n_top), dtype=T.float32)
+    with _new_on(stream, dev):
+        logprob = None if targets is None else logits.new_empty(rows, dtype=T.float32)
+        entropy = logits.new_empty(rows, dtype=T.float32)
+        if n_top > 0:
+            ids = logits.new_empty((rows, n_top), dtype=T.int32)
+            top = logits.new_empty((rows, n_top), dtype=T.float32)
     _check(lib().s2k_logprobs(dev, logits.data_ptr(), code, rows, n, max(logits.stride(0), 0), tgt, n_top,
                               None if logprob is None else logprob.data_ptr(), entropy.data_ptr(),
                               None if ids is None else ids.data_ptr(), None if top is None else top.data_ptr(),

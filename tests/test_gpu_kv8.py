@@ -399,3 +399,29 @@ def test_binding_refusals():
                 lambda: s2k.KV8Cache(c.cache.k.cpu(), c.cache.v, c.cache.k_scale, c.cache.v_scale)):
         with pytest.raises(s2k.S2KError):
             bad()
+
+
+def test_results_belong_to_the_stream_that_writes_them():
+    """Memory that the current stream gave back, and may still be using, is not handed to another stream's call."""
+    c = Call([1], [40], 8, 2, 128, "f32")
+    q = c.heads(8)
+    side = torch.cuda.Stream()
+    x = torch.randn(1, 1000, device="cuda")
+
+    def results(stream):
+        k, v = c.cache.read(c.layer, 1, *c.args, stream=stream)
+        ids = s2k.logprobs(x, torch.zeros(1, dtype=torch.int32, device="cuda"), 4, stream=stream)
+        return [c.cache.attend(c.layer, q, *c.args, stream=stream), k, v, *ids]
+
+    torch.cuda.synchronize()
+    kept = results(None)
+    want = [t.clone() for t in kept]
+    torch.cuda.synchronize()
+    ours = {t.untyped_storage().data_ptr() for t in kept}
+    del kept
+    for stream in (side, side.cuda_stream):
+        got = results(stream)
+        torch.cuda.synchronize()
+        assert not ours & {t.untyped_storage().data_ptr() for t in got}
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del got
