@@ -6,6 +6,7 @@
 #include "s2k_kv8.h"
 #include "s2k_model.h"
 
+#include <algorithm>
 #include <atomic>
 #include <climits>
 #include <cmath>
@@ -42,6 +43,8 @@ struct OnDevice {
         if (before >= 0) cudaSetDevice(before);
     }
 };
+
+constexpr double kMaxExtent = (double)((int64_t)1 << 40);  // elements from a tensor's first to its last
 
 int elem_size(int type) { return type == S2K_TYPE_F32 ? 4 : type == S2K_TYPE_F16 || type == S2K_TYPE_BF16 ? 2 : 0; }
 
@@ -99,6 +102,9 @@ s2k_status check_heads(const char *what, const s2k_heads *t, const Kv8Rows &r, i
     if (!t->data && r.n_rows > 0) return fail(S2K_ERR_ARG, "NULL %s", what);
     if ((uintptr_t)t->data % es) return fail(S2K_ERR_ARG, "%s is not aligned to its elements", what);
     if (t->row_stride < 0 || t->head_stride < 0) return fail(S2K_ERR_ARG, "%s has a negative stride", what);
+    // no memory is that large, and every offset stays within 64 bits
+    if ((double)t->row_stride * std::max(r.n_rows - 1, 0) + (double)t->head_stride * (n_heads - 1) > kMaxExtent)
+        return fail(S2K_ERR_ARG, "%s reaches too far", what);
     if (written) {
         // [rows][heads][dim] or [heads][rows][dim], each with gaps or without
         const int64_t rs = t->row_stride, hs = t->head_stride;

@@ -438,6 +438,8 @@ class SlowARModel:
     def init_kv8_cache(self, max_seq_len: int, window: int = 0, sinks: int = 0) -> None:
         """A KV cache in 8 bits, with attention to the last `window` (0: all) and the first `sinks` positions
         (s2k_seq_create_kv8)."""
+        if (max_seq_len | window | sinks) >> 31:
+            _not_int32("max_seq_len, window or sinks", max_seq_len, window, sinks)
         self.clear_kv_cache()
         _check(lib().s2k_seq_create_kv8(self._m, max_seq_len, window, sinks, ctypes.byref(self._seq)))
         self._max_seq_len = max_seq_len
@@ -482,6 +484,8 @@ class SlowARModel:
         flat = np.ascontiguousarray(flat_tokens, dtype=np.int32)
         if flat.size != n_tokens * (self._hp.num_codebooks + 1):
             raise S2KError(-1, f"expected {n_tokens * (self._hp.num_codebooks + 1)} ints, got {flat.size}")
+        if n_top >> 31:
+            _not_int32("n_top", n_top)
         lp, ent = np.empty(max(n_tokens - 1, 0), np.float32), np.empty(n_tokens, np.float32)
         k = max(n_top, 0)
         ids, top = np.empty((n_tokens, k), np.int32), np.empty((n_tokens, k), np.float32)
@@ -937,6 +941,11 @@ def _op_type(what: str, t) -> int:
     return code
 
 
+def _not_int32(what: str, *values):
+    # ctypes would cut them to 32 bits without a word
+    raise S2KError(-1, f"{what} out of range: {', '.join(map(str, values))}")
+
+
 def _op_stream(device: int, stream) -> int:
     return _raw_stream(device) if stream is None else int(getattr(stream, "cuda_stream", stream))
 
@@ -1016,6 +1025,8 @@ class KV8Cache:
             if row_start is not None or n <= 0 or n_rows % n:
                 raise S2KError(-1, "max_rows is needed where rows are not shared out evenly")
             max_rows = n_rows // n
+        if (n | n_rows | max_rows | ld) >> 31:
+            _not_int32("sequences, rows, max_rows or table entries", n, n_rows, max_rows, ld)
         return _PACK_ROWS(n, n_rows, max_rows, ld, _ints("past", past, (n,), dev),
                           0 if row_start is None else _ints("row_start", row_start, (n + 1,), dev),
                           _ints("block_table", block_table, shape, dev),
@@ -1037,6 +1048,8 @@ class KV8Cache:
         """Stores rows [rows][kv_heads][head_dim] of keys and values (s2k_kv8_append)."""
         if k.shape != v.shape:
             raise S2KError(-1, "k and v have different shapes")
+        if layer >> 31:
+            _not_int32("layer", layer)
         r = self._rows(k.shape[0], past, block_table, row_start, max_rows, err)
         kh, vh = self._heads("k", k, self.n_kv_heads), self._heads("v", v, self.n_kv_heads)
         _check(lib().s2k_kv8_append(self._c, layer, r, kh, vh, _op_stream(self.device, stream)))
@@ -1045,6 +1058,8 @@ class KV8Cache:
              dtype=None, out=None, err=None, stream=None):
         """(k, v) [n_rows][kv_heads][head_dim] that the rows' positions hold, float32 or `dtype`, or written to
         the pair `out` (s2k_kv8_read)."""
+        if (layer | n_rows) >> 31:
+            _not_int32("layer or rows", layer, n_rows)
         if out is None:
             shape = (n_rows, self.n_kv_heads, self.head_dim)
             dtype = self.k_scale.dtype if dtype is None else dtype
@@ -1062,6 +1077,8 @@ class KV8Cache:
         """Attention of rows q [rows][heads][head_dim] over their sequences' cached positions, causal, with the
         last `window` keys (0: all) and the first `sinks` keys visible (s2k_kv8_attend); scale defaults to
         head_dim ** -0.5.  Returns out, a tensor like q unless given."""
+        if (layer | window | sinks) >> 31:
+            _not_int32("layer, window or sinks", layer, window, sinks)
         qh = self._heads("q", q, None)
         if out is None:
             if stream is None:
@@ -1087,6 +1104,8 @@ def logprobs(logits, targets=None, n_top: int = 0, stream=None):
     if logits.dim() != 2 or logits.shape[1] == 0 or (logits.shape[0] and logits.stride(1) != 1):
         raise S2KError(-1, "logits must be [rows][n] with a dense last dimension")
     rows, n = logits.shape
+    if (rows | n | n_top) >> 31:
+        _not_int32("rows, logits or n_top", rows, n, n_top)
     dev, code = logits.get_device(), _op_type("logits", logits)
     if dev < 0:
         raise S2KError(-1, "logits is not on a CUDA device")

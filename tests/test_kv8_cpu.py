@@ -132,3 +132,34 @@ def test_plain_append_by_steps_stays_near_one_call():
     assert s1[0, 0, 0] == s2[0, 0, 0]
     d = np.abs(ku.values(steps, s2, 0, t[0], 16, False) - x)
     assert d.max() <= s2[0, 0, 0] * (0.5 * grew + 0.01)
+
+
+@pytest.mark.skipif(s2k.device_count() > 0, reason="fake addresses: only where nothing can be launched")
+def test_strides_whose_extents_pass_64_bits():
+    far = 1 << 62
+    many = rows(n_seqs=1, n_rows=9, max_rows=9)
+    for bad in (heads(row_stride=far), heads(head_stride=far)):
+        assert call(r=many, k=bad) == call(r=many, k=bad, fn="s2k_kv8_read") == ARG
+    assert attend(r=many, out=heads(4, row_stride=128, head_stride=far)) == ARG
+    assert attend(r=many, out=heads(4, row_stride=far, head_stride=128)) == ARG
+    assert call(k=heads(row_stride=1 << 30)) == NO_DEVICE
+    assert call(k=heads(row_stride=128, head_stride=1 << 34)) == NO_DEVICE  # [heads][rows][dim] of many rows
+
+
+def test_numbers_beyond_32_bits_are_not_cut():
+    """ctypes would pass 2^32 + 5 as 5."""
+    torch = pytest.importorskip("torch")
+    c = object.__new__(s2k.KV8Cache)
+    s2k._torch_module()
+    c.device, c.n_pages, c.n_layers, c.n_kv_heads, c.head_dim, c._c = 0, 1, 1, 1, 64, b""
+    c.k_scale = torch.zeros(1)
+    q, past, table = torch.zeros(1, 1, 64), torch.zeros(1, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32)
+    big = (1 << 32) + 5
+    for f in (lambda: c.append(big, q, q, past, table), lambda: c.read(big, 1, past, table),
+              lambda: c.read(0, big, past, table),
+              lambda: c.attend(big, q, past, table), lambda: c.attend(0, q, past, table, window=big),
+              lambda: c.attend(0, q, past, table, sinks=big), lambda: c._rows(1, past, table, past, big, None),
+              lambda: s2k.logprobs(torch.zeros(1, 64), n_top=big),
+              lambda: s2k.logprobs(torch.zeros(1, 1).expand(big, 1))):
+        with pytest.raises(s2k.S2KError, match="out of range"):
+            f()
