@@ -584,8 +584,8 @@ S2K_API int64_t s2k_codec_stream_max_release(const s2k_codec_stream *s);
 
 /* A paged KV cache in 8 bits.  A page holds 16 tokens of every (layer, kv
  * head); a value stands for its int8 (in [-127, 127]) times its block's scale,
- * a block being one page of one layer and kv head.  k and v 16-byte aligned;
- * head_dim 64 or 128. */
+ * a block being one page of one layer and kv head.  Scales are not negative
+ * (NaN: the block reads as NaN).  k and v 16-byte aligned; head_dim 64 or 128. */
 typedef struct s2k_kv8 {
     int8_t *k;      /* [n_pages][n_layers][n_kv_heads][16][head_dim] */
     int8_t *v;      /* [n_pages][n_layers][n_kv_heads][head_dim][16]: transposed */
@@ -601,8 +601,9 @@ typedef struct s2k_kv8 {
  * are read on the device when the call runs.  A sequence whose entries do not
  * fit (a negative count or past, more than max_rows rows, rows beyond n_rows,
  * positions beyond the table) is skipped, and so is a page that is none of the
- * cache's; each sets bit 8 of *err where err is given.  Rows of no sequence
- * are neither read nor written. */
+ * cache's; each ors 8 into *err where err is given.  (s2k_kv8_attend ors 1 or 2 into
+ * it if a bounded wait of its own ran out; its rows are then not valid.)  Rows
+ * of no sequence are neither read nor written. */
 typedef struct s2k_kv8_rows {
     int32_t n_seqs, n_rows;
     int32_t max_rows;           /* most rows of one sequence */
@@ -642,7 +643,7 @@ S2K_API s2k_status s2k_kv8_read(const s2k_kv8 *c, int32_t layer, const s2k_kv8_r
  * over the keys j <= p of the row's position p with window == 0, or
  * j > p - window (the last `window` keys), or j < sinks (the first ones).
  * n_heads query heads share the kv heads in groups of n_heads / n_kv_heads.
- * q and out have the same type; out may be q.  Sums and softmax statistics
+ * q and out have the same type; out is q itself or does not overlap it.  Sums and softmax statistics
  * are f32.  A row that sees no key (all its pages skipped) is zero. */
 S2K_API s2k_status s2k_kv8_attend(const s2k_kv8 *c, int32_t layer, const s2k_kv8_rows *r, const s2k_heads *q,
                                   const s2k_heads *out, int32_t n_heads, float scale, int32_t window, int32_t sinks,

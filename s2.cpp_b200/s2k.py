@@ -985,7 +985,7 @@ class KV8Cache:
     [n_seqs][entries] page numbers, row_start [n_seqs + 1] first row of each
     sequence (None: the rows are shared out evenly), max_rows the most rows of
     one sequence.  These three are int32 CUDA tensors that the kernels read.  An
-    optional int32 tensor `err` gets bit 8 set where an entry does not fit (see
+    optional int32 tensor `err` gets 8 or-ed in where an entry does not fit (see
     s2k_kv8_rows); such rows, and rows of no sequence, are left unwritten."""
 
     PAGE = 16
