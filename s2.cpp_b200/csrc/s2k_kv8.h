@@ -239,6 +239,8 @@ struct Kv8Attn {
 
 cudaError_t launch_kv8_append(const Kv8 &c, const Kv8Rows &r, const Rows &k, const Rows &v, cudaStream_t st);
 cudaError_t launch_kv8_read(const Kv8 &c, const Kv8Rows &r, const Rows &k, const Rows &v, cudaStream_t st);
+// slots of a CTA of the prompt kernel
+constexpr int kv8_prompt_slots(int type) { return type == OT_F32 ? 128 : 256; }
 cudaError_t launch_kv8_attend(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, cudaStream_t st);
 
 // the same for calls of many rows per sequence

@@ -1,5 +1,5 @@
 // s2k_kv8_attn.cu -- attention of few query rows over the 8-bit paged KV cache
-// (decode steps, drafted tokens); prompts run in s2k_kv8_prompt.cu.
+// (decode steps, drafted tokens, short prompts); s2k_kv8_prompt.cu has the rest.
 //
 //   o = sum_j w_j v_j,  w = softmax over the visible keys of scale * q.k_j
 // Row i of a sequence sits at position p = past + i and sees key j iff
@@ -485,7 +485,6 @@ static cudaError_t decode_launch(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &
 cudaError_t launch_kv8_attend(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, cudaStream_t st) {
     if (r.n_seqs == 0 || r.max_rows == 0) return cudaSuccess;
     const int G = a.n_heads / c.n_kv_heads;
-    if ((long long)r.max_rows * G > 64) return launch_kv8_prompt(c, r, a, st);
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
@@ -501,12 +500,26 @@ cudaError_t launch_kv8_attend(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, 
         d.sms = sms;
         d.ready.store(1, std::memory_order_release);
     }
-    const int slots = a.q.type == OT_F32 ? Digits<OT_F32>::slots : Digits<OT_F16>::slots;
-    const int tiles = (r.max_rows * G + slots - 1) / slots;
-    const long long units = (long long)tiles * c.n_kv_heads * r.n_seqs;
-    // pages of one unit at most
-    long long pages = r.table_ld;
-    if (a.window) pages = std::min(pages, ((long long)a.window + r.max_rows + a.sinks) / kPage + 3);
+    // tiles of `per` slots of a (sequence, kv head), and the pages that one of them sees at most
+    auto tiles_of = [&](long long per) { return ((long long)r.max_rows * G + per - 1) / per; };
+    auto pages_of = [&](long long per) {
+        const long long rows = std::min<long long>(r.max_rows, per / G + 2);
+        const long long seen = a.window ? ((long long)a.window + rows + a.sinks) / kPage + 3 : r.table_ld;
+        return std::min<long long>(seen, r.table_ld);
+    };
+    const long long slots = a.q.type == OT_F32 ? Digits<OT_F32>::slots : Digits<OT_F16>::slots;
+    const long long tiles = tiles_of(slots), pages = pages_of(slots);
+    const long long groups = (long long)c.n_kv_heads * r.n_seqs, units = tiles * groups;
+    // Which kernel.  Here every tile of 4 or 8 slots walks the pages, spread over the SMs: a page of a tile is the unit
+    // of time, a tile's start about 30 of them.  The prompt kernel walks them once for 128 or 256 slots, one CTA per SM:
+    // wave by wave a page takes 3 units, its start and end about 80 pages.  The wrong one is up
+    // to 17 times slower (one f32 sequence of 16000 tokens, 64 slots, 8 heads: 104 us here, 275 there; 64 sequences of 2500:
+    // 780 and 286; of 8 slots: 115 and 266; one of 100 with 64 slots: 4.5 and 12.7).  Over 920 calls of both kernels the
+    // choice is 0.3 % from the better one on average and 23 % at most.
+    const long long prompt_slots = kv8_prompt_slots(a.q.type);
+    const long long waves = (tiles_of(prompt_slots) * groups + d.sms - 1) / d.sms;
+    if (tiles > 65535 || (double)units * (pages + 30) > 3.0 * d.sms * waves * (pages_of(prompt_slots) + 80))
+        return launch_kv8_prompt(c, r, a, st);
     // CTAs per unit.  A CTA's start and its join cost about as much as 40 pages: pieces of about 64 pages are best
     // where the machine is full (64 sequences of up to 2523 tokens: 46 us whole, 43.6 halved, 48 in thirds; 8 of up
     // to 6095: 20.6 in fourths, 18.9 in sixths, 24.2 in sevenths; 16 of 4000 visible ones: 18.4 in thirds, 16.4 in
@@ -518,7 +531,7 @@ cudaError_t launch_kv8_attend(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, 
     if ((long long)r.n_seqs * cs > 0x7fffffffLL) return cudaErrorInvalidValue;
     count_launch();
     return kv8_dispatch(c.head_dim, a.q.type, [&](auto hd, auto type) {
-        return decode_launch<hd, type>(c, r, a, cs, tiles, st);
+        return decode_launch<hd, type>(c, r, a, cs, (int)tiles, st);
     });
 }
 

@@ -149,7 +149,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
     using T = typename OType<TYPE>::T;
     using Sm = PromptSmem<HD>;
     constexpr bool wide = TYPE == OT_F32;
-    constexpr int NC = Sm::NC, SLOTS = wide ? kPM : 2 * kPM;
+    constexpr int NC = Sm::NC, SLOTS = kv8_prompt_slots(TYPE);
+    static_assert(SLOTS == (wide ? kPM : 2 * kPM), "groups of kPM slots");
     constexpr unsigned kAll = 0xffffffffu;
     extern __shared__ uint8_t raw[];
     Sm &sm = *reinterpret_cast<Sm *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -775,7 +776,7 @@ cudaError_t launch_kv8_prompt(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, 
         g_prompt_ready[dev].store(1, std::memory_order_release);
     }
     const long long slots = (long long)r.max_rows * (a.n_heads / c.n_kv_heads);
-    const int per = a.q.type == OT_F32 ? kPM : 2 * kPM;
+    const int per = kv8_prompt_slots(a.q.type);
     const long long tiles = (slots + per - 1) / per;
     if (slots > 0x7fffffffLL || tiles * r.n_seqs > 0x7fffffffLL) return cudaErrorInvalidValue;
     const dim3 grid((unsigned)(tiles * r.n_seqs), c.n_kv_heads);

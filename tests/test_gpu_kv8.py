@@ -425,3 +425,35 @@ def test_results_belong_to_the_stream_that_writes_them():
         assert not ours & {t.untyped_storage().data_ptr() for t in got}
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         del got
+
+
+# Which kernel a call takes depends on how much there is to do per SM: the calls above are small, these are the same
+# cases at sizes that the prompt kernel gets (many sequences, most of them without rows, or more rows).
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (50, 0), (37, 5), (16, 40), (100000, 3)])
+@pytest.mark.parametrize("rows,past,H,Hkv,D", PROMPTS)
+def test_attend_of_a_crowd(rows, past, H, Hkv, D, window, sinks, typ):
+    test_attend(rows + [0] * 200, past + [0] * 200, H, Hkv, D, window, sinks, typ)
+
+
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+def test_attend_strides_scale_and_in_place_of_many_rows(typ):
+    test_attend_strides_scale_and_in_place([900], typ)
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16"])
+def test_attend_hidden_blocks_of_many_rows(typ):
+    test_attend_hidden_blocks_may_hold_anything([1500], [300], typ)
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+def test_attend_negative_scale_and_odd_queries_of_many_rows(typ):
+    test_attend_negative_scale_and_odd_queries([1000], typ)
+
+
+def test_attend_far_scores_of_many_rows():
+    test_attend_far_scores_scales_and_not_a_number(400)
+
+
+def test_bad_entries_of_many_rows():
+    test_bad_entries_are_skipped_and_told(400)
