@@ -9,10 +9,13 @@
 // (the running maximum of 16 values changes about 3.4 times on average).
 //
 // The quotient is rounded exactly: the product with 1/s is within 127 * 2^-23 =
-// 1.5e-5 of it, so only a result that near to a half is divided again, in
-// double (where a 24-bit by 24-bit quotient that is no half stays at least
-// 2^-33 away from one).  The stored integers are then a function of the inputs
-// alone, whatever computes them.
+// 1.5e-5 of it, so its nearest integer n is right or one off, and the remainder
+// e = x - n s tells: n is right iff |e| < s/2 (or = and n is even).  One fma
+// gives e exactly: it is a multiple of s's last place (for n = 0 it is x) and
+// not larger than about s/2, so it fits 24 bits.  The stored integers are then a
+// function of the inputs alone, whatever computes them.  (Before, quotients
+// near a half were divided again in double.  16-bit inputs have one in nearly
+// every block: eight prompts of bf16 rows took 123 us, f32 ones 67.)
 //
 // int8 with a block's scale rather than an 8-bit float: over a block of normal
 // values the uniform step's error is about a third of e4m3's, and every
@@ -21,7 +24,8 @@
 // A block with a NaN or an infinity gets a NaN scale: it reads as NaN.
 //
 // Measured: eight prompts of up to 4096 f32 rows, 8 heads of 128, stored and read
-// back: 95 us (4.88 TB/s), 55 us and 39 us in the kernels.
+// back: 91 us (5.1 TB/s), 49 us and 40 us in the kernels.  One token: 2.7 and 2.4
+// us in the kernels, replayed one after another.
 #include "s2k_common.cuh"
 #include "s2k_kv8.h"
 
@@ -33,28 +37,27 @@ constexpr int kKv8Warps = 4;
 // rounding instructions run at a quarter of an addition's rate.
 constexpr float kRound = 12582912.f;
 
-// round(a * b / s), b = 1 or an older scale; kept out of line: 64 divisions in double in the loop's code made the
-// instruction cache the bound (124 us for eight prompts).
-__device__ __noinline__ unsigned q8_exact(float a, float b, float s) {
-    return s == 0.f ? 0u : (unsigned)(int)fmin(fmax(rint((double)a * (double)b / (double)s), -127.0), 127.0);
+// round(x / s) in the low byte, inv = 1 / s; s >= 2^-110 or s = x = 0
+__device__ __forceinline__ unsigned q8(float x, float s, float inv) {
+    const float t = __fadd_rn(__fmul_rn(x, inv), kRound);
+    const int n = __float_as_int(t), e = __float_as_int(fmaf(-__fsub_rn(t, kRound), s, x));
+    // |e| > s/2, or = and n is odd, in the order of their bits
+    return (e & 0x7fffffff) + (n & 1) > __float_as_int(0.5f * s) ? n + (e >> 31 | 1) : n;
 }
-// q = round(r) in the low byte; far: the largest distance of an r from its integer so far
-__device__ __forceinline__ unsigned q8_fast(float r, float &far) {
-    const float t = __fadd_rn(r, kRound);
-    far = fmaxf(far, fabsf(__fsub_rn(r, __fsub_rn(t, kRound))));
-    return __float_as_uint(t);
-}
-// q = round(a * b / s) in the low byte; r is the quotient to 1.5e-5
-__device__ __forceinline__ unsigned q8_careful(float r, bool tiny, float a, float b, float s) {
-    float far = 0.f;
-    const unsigned q = q8_fast(r, far);
-    return tiny || far > 0.49998f ? q8_exact(a, b, s) : q;
+// round(q * was / s) for an older token's q, ratio = was / s: near a half it is divided in double, where a 31-bit by
+// 24-bit quotient that is no half stays at least 2^-33 away from one
+__device__ __forceinline__ unsigned q8_again(float q, float was, float s, float ratio) {
+    const float r = __fmul_rn(q, ratio), t = __fadd_rn(r, kRound);
+    if (s >= 1.17549435e-38f && fabsf(__fsub_rn(r, __fsub_rn(t, kRound))) <= 0.49998f) return __float_as_uint(t);
+    return (unsigned)(int)fmin(fmax(rint((double)q * (double)was / (double)s), -127.0), 127.0);
 }
 
 // the low bytes of four words
 __device__ __forceinline__ unsigned low_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
+// the first n bytes of a word
+__device__ __forceinline__ unsigned byte_mask(int n) { return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1u; }
 // byte i of w as a number, exactly: 128 + q under 2^23's exponent
 __device__ __forceinline__ float byte_value(unsigned w, int i) {
     return __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7440 + i)) - 8388736.f;
@@ -63,10 +66,13 @@ __device__ __forceinline__ float byte_value(unsigned w, int i) {
 // One warp per (sequence, page, kv head, keys or values): lane l holds dims
 // [l*D, l*D + D) of the page's 16 tokens, so the block's maximum is one warp
 // reduction and nothing is read twice.  Bound by the rows' bytes for prompts,
-// by the chain of dependent loads for a single token.
+// by the chain of dependent loads for a single token.  Five CTAs per SM (96
+// registers, a few of them spilled): 8 x 4096 f32 rows of 8 heads of 128 take 60
+// us (5.6 TB/s), bf16 ones 57; with the compiler's choice of 168, 72 and 71.  One
+// token 3.0 us against 2.6, one of 64 sequences 3.7, of 256 6.7 against 8.0.
 template <int HD, int TYPE, bool VEC>
-__global__ void __launch_bounds__(kKv8Warps * 32) kv8_append_kernel(Kv8 c, Kv8Rows r, Rows k, Rows v,
-                                                                   int pages_per_seq) {
+__global__ void __launch_bounds__(kKv8Warps * 32, 5) kv8_append_kernel(Kv8 c, Kv8Rows r, Rows k, Rows v,
+                                                                      int pages_per_seq) {
     using T = typename OType<TYPE>::T;
     constexpr int D = HD / 32;
     const int lane = threadIdx.x & 31;
@@ -102,82 +108,87 @@ __global__ void __launch_bounds__(kKv8Warps * 32) kv8_append_kernel(Kv8 c, Kv8Ro
     const bool bad = top >= 0x7f800000u || was != was;
     const float fresh = __fdiv_rn(amax, 127.f);
     const float s = bad ? __int_as_float(0x7fc00000) : fmaxf(fresh, was);
-    const bool zero = bad || s == 0.f, tiny = s < 1.17549435e-38f;
-    const float inv = zero ? 0.f : __fdiv_rn(1.f, s);
-    const bool again = lo > 0 && s != was && !zero;  // the older tokens' scale grew
-    const float ratio = again ? __fdiv_rn(was, s) : 1.f;
-    if (bad) {  // x * 0 would keep a NaN
+    const bool zero = bad || s == 0.f, tiny = s < 7.8886091e-31f;  // 2^-100
+    const float su = zero ? 0.f : tiny ? s * 18446744073709551616.f : s;
+    if (zero || tiny) {
+        // a NaN or an infinity would stay one; far down, both sides by 2^64, exactly.  A subnormal scale is so coarse that
+        // a quotient can pass 127.
+        const float most = 127.f * su;
 #pragma unroll
         for (int t = 0; t < kPage; ++t)
 #pragma unroll
-            for (int d = 0; d < D; ++d) x[t][d] = 0.f;
+            for (int d = 0; d < D; ++d)
+                x[t][d] = zero ? 0.f : fminf(fmaxf(x[t][d] * 18446744073709551616.f, -most), most);
     }
-    // D of a key's bytes, or 16 of a value's dimension, are words of four.  The first pass rounds without a branch; a
-    // lane that was too near to a half somewhere (one in 400) goes over its values again, as does every lane where older
-    // tokens are rounded again.
-    float far = 0.f;
-    auto pass = [&](auto careful) {
-        auto quant = [&](float y) {
-            const float r = __fmul_rn(y, inv);
-            return careful ? q8_careful(r, tiny, y, 1.f, zero ? 0.f : s) : q8_fast(r, far);
+    const float inv = zero ? 0.f : __fdiv_rn(1.f, su);
+    if (lo > 0 && s != was && !zero) {  // the older tokens' scale grew: 4 or 16 bytes at a time, rarely and compactly
+        const float ratio = __fdiv_rn(was, s);
+        auto again = [&](unsigned w) {
+            unsigned y = 0;
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) y = __funnelshift_r(y, q8_again(byte_value(w, i), was, s, ratio), 8);
+            return y;
         };
-        auto requant = [&](unsigned w, int i) {
-            const float q = byte_value(w, i);
-            return q8_careful(__fmul_rn(q, ratio), tiny, q, was, s);
-        };
-        const bool older_too = careful && again;
         if (!is_v) {
-#pragma unroll
-            for (int t = 0; t < kPage; ++t) {
+            // a lane's D bytes of a key; the two of head_dim 64 as the low half of a word
+#pragma unroll 1
+            for (int t = 0; t < lo; ++t) {
                 unsigned char *at = reinterpret_cast<unsigned char *>(dst + t * HD + lane * D);
-                unsigned w;
-                if (t >= lo && t < hi) {
-                    w = low_bytes(quant(x[t][0]), quant(x[t][1]), D == 4 ? quant(x[t][D - 2]) : 0u, D == 4 ? quant(x[t][D - 1]) : 0u);
-                } else if (t < lo && older_too) {
-                    const unsigned o = D == 4 ? *reinterpret_cast<const unsigned *>(at) : *reinterpret_cast<const uint16_t *>(at);
-                    w = low_bytes(requant(o, 0), requant(o, 1), D == 4 ? requant(o, 2) : 0u, D == 4 ? requant(o, 3) : 0u);
-                } else {
-                    continue;
-                }
-                if (D == 4) *reinterpret_cast<unsigned *>(at) = w;
-                else *reinterpret_cast<uint16_t *>(at) = (uint16_t)w;
+                if (D == 4) *reinterpret_cast<unsigned *>(at) = again(*reinterpret_cast<const unsigned *>(at));
+                else *reinterpret_cast<uint16_t *>(at) = (uint16_t)again(*reinterpret_cast<const uint16_t *>(at));
             }
         } else {
-#pragma unroll
-            for (int d = 0; d < D; ++d) {
-                uint4 *at = reinterpret_cast<uint4 *>(dst + (lane * D + d) * kPage);
-                unsigned w[4] = {};
-                const bool part = lo > 0 || hi < kPage;
-                if (part) {
-                    const uint4 o = *at;
-                    w[0] = o.x, w[1] = o.y, w[2] = o.z, w[3] = o.w;
-                }
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    unsigned q[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) q[e] = quant(x[4 * g + e][d]);
-                    const unsigned fresh = low_bytes(q[0], q[1], q[2], q[3]);
-                    if (!part) {
-                        w[g] = fresh;
-                        continue;
-                    }
-                    if (older_too && 4 * g < lo) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) q[e] = requant(w[g], e);
-                    }
-                    const unsigned older = older_too && 4 * g < lo ? low_bytes(q[0], q[1], q[2], q[3]) : w[g];
-                    // bytes [lo, hi) are new, those before older, those behind stay
-                    auto mask = [&](int n) { return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1u; };
-                    const unsigned m_old = mask(lo - 4 * g), m_new = mask(hi - 4 * g) & ~m_old;
-                    w[g] = (older & m_old) | (fresh & m_new) | (w[g] & ~(m_old | m_new));
-                }
-                *at = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll 1
+            for (int g = 0; g < 4 * D; ++g) {  // four tokens of a dimension; those behind lo are new or unused
+                if (g % 4 * 4 >= lo) continue;
+                unsigned *at = reinterpret_cast<unsigned *>(dst + (lane * D + g / 4) * kPage) + g % 4;
+                const unsigned w = *at, m = byte_mask(lo - g % 4 * 4);
+                *at = (again(w) & m) | (w & ~m);
             }
         }
-    };
-    if (!tiny && !again) pass(std::false_type());
-    if (tiny || again || far > 0.49998f) pass(std::true_type());
+    }
+    if (!is_v) {
+#pragma unroll
+        for (int t = 0; t < kPage; ++t) {
+            if (t < lo || t >= hi) continue;
+            unsigned char *at = reinterpret_cast<unsigned char *>(dst + t * HD + lane * D);
+            unsigned q[D];
+#pragma unroll
+            for (int d = 0; d < D; ++d) q[d] = q8(x[t][d], su, inv);
+            if (D == 4) *reinterpret_cast<unsigned *>(at) = low_bytes(q[0], q[1], q[D - 2], q[D - 1]);
+            else *reinterpret_cast<uint16_t *>(at) = (uint16_t)low_bytes(q[0], q[1], 0u, 0u);
+        }
+    } else {
+        // 16 bytes of a dimension: four words of four tokens
+        if (lo == 0 && hi == kPage) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                unsigned w[4];
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    w[g] = low_bytes(q8(x[4 * g][d], su, inv), q8(x[4 * g + 1][d], su, inv), q8(x[4 * g + 2][d], su, inv),
+                                     q8(x[4 * g + 3][d], su, inv));
+                *reinterpret_cast<uint4 *>(dst + (lane * D + d) * kPage) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            if (lane == 0) *scale = s;
+            return;
+        }
+        // part of a page: bytes [lo, hi) are new, the others stay
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const unsigned m = byte_mask(hi - 4 * g) & ~byte_mask(lo - 4 * g);
+            if (!m) continue;
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                unsigned *at = reinterpret_cast<unsigned *>(dst + (lane * D + d) * kPage) + g;
+                unsigned q[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[e] = q8(x[4 * g + e][d], su, inv);
+                const unsigned w = low_bytes(q[0], q[1], q[2], q[3]);
+                *at = (w & m) | (*at & ~m);
+            }
+        }
+    }
     if (lane == 0 && (lo == 0 || s != was)) *scale = s;
 }
 

@@ -457,3 +457,31 @@ def test_attend_far_scores_of_many_rows():
 
 def test_bad_entries_of_many_rows():
     test_bad_entries_are_skipped_and_told(400)
+
+
+@pytest.mark.parametrize("bits", [1, 2, 4, 7])
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+def test_append_of_few_mantissa_bits(typ, bits):
+    """Values and maxima of few bits, whose quotients are halves or next to one nearly everywhere, from the smallest
+    magnitudes of the type to large ones; page by page in one call, then in parts."""
+    rows, D, Hkv = [16 * 24], 128, 2
+    rng = np.random.default_rng(bits)
+    lo, hi = {"f32": (-149, 100), "f16": (-24, 14), "bf16": (-133, 100)}[typ]
+    c = Call(rows, [0], 4, Hkv, D, typ)
+    m = rng.integers(-(2 ** bits), 2 ** bits + 1, (rows[0], Hkv, D)).astype(np.float64)
+    e = np.repeat(rng.integers(lo, hi - bits, (24, Hkv, 1)), 16, 0)
+    k = torch.from_numpy(np.ldexp(m, e)).to(DT[typ]).cuda()
+    v = k.flip(2).contiguous()
+    assert torch.isfinite(k).all()
+    for parts in ([rows[0]], [5, 16, 1, 6, rows[0] - 28]):
+        at = 0
+        for n in parts:
+            past = i32([at])
+            x, y = k[at:at + n].contiguous(), v[at:at + n].contiguous()
+            c.cache.append(c.layer, x, y, past, c.args[1])
+            ku.append(c.kq, c.ks, c.layer, x.double().cpu().numpy(), [0, n], [at], c.table, False)
+            ku.append(c.vq, c.vs, c.layer, y.double().cpu().numpy(), [0, n], [at], c.table, True)
+            at += n
+        assert np.array_equal(c.cache.k_scale.cpu().numpy(), c.ks, equal_nan=True)
+        assert np.array_equal(c.cache.v_scale.cpu().numpy(), c.vs, equal_nan=True)
+        assert np.array_equal(c.cache.k.cpu().numpy(), c.kq) and np.array_equal(c.cache.v.cpu().numpy(), c.vq)
