@@ -648,6 +648,10 @@ S2K_API s2k_status s2k_kv8_read(const s2k_kv8 *c, int32_t layer, const s2k_kv8_r
 S2K_API s2k_status s2k_kv8_attend(const s2k_kv8 *c, int32_t layer, const s2k_kv8_rows *r, const s2k_heads *q,
                                   const s2k_heads *out, int32_t n_heads, float scale, int32_t window, int32_t sinks,
                                   void *stream);
+/* Test hook: which kernel this thread's last attention over an 8-bit cache
+ * (s2k_kv8_attend or a model's) took: 1 the one for few rows, 2 the one for
+ * many, 0 none yet. */
+S2K_API int32_t s2k_debug_kv8_attend_kernel(void);
 
 /* Most alternatives of s2k_logprobs. */
 #define S2K_LOGPROBS_MAX_TOP 32

@@ -243,6 +243,9 @@ cudaError_t launch_kv8_read(const Kv8 &c, const Kv8Rows &r, const Rows &k, const
 constexpr int kv8_prompt_slots(int type) { return type == OT_F32 ? 128 : 256; }
 cudaError_t launch_kv8_attend(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, cudaStream_t st);
 
+// this thread's last launch_kv8_attend: 1 the kernel of few rows, 2 that of many
+extern thread_local int g_kv8_attend_kernel;
+
 // the same for calls of many rows per sequence
 cudaError_t launch_kv8_prompt(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, cudaStream_t st);
 

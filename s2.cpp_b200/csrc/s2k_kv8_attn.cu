@@ -451,6 +451,8 @@ struct DecodeDevice {
 };
 static DecodeDevice g_decode[64];
 
+thread_local int g_kv8_attend_kernel = 0;
+
 template <int HD, int TYPE>
 static constexpr int decode_smem() {
     return (int)sizeof(DecodeSmem<HD, Digits<TYPE>::slots>) + 128;
@@ -518,8 +520,11 @@ cudaError_t launch_kv8_attend(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, 
     // choice is 0.3 % from the better one on average and 23 % at most.
     const long long prompt_slots = kv8_prompt_slots(a.q.type);
     const long long waves = (tiles_of(prompt_slots) * groups + d.sms - 1) / d.sms;
-    if (tiles > 65535 || (double)units * (pages + 30) > 3.0 * d.sms * waves * (pages_of(prompt_slots) + 80))
+    if (tiles > 65535 || (double)units * (pages + 30) > 3.0 * d.sms * waves * (pages_of(prompt_slots) + 80)) {
+        g_kv8_attend_kernel = 2;
         return launch_kv8_prompt(c, r, a, st);
+    }
+    g_kv8_attend_kernel = 1;
     // CTAs per unit.  A CTA's start and its join cost about as much as 40 pages: pieces of about 64 pages are best
     // where the machine is full (64 sequences of up to 2523 tokens: 46 us whole, 43.6 halved, 48 in thirds; 8 of up
     // to 6095: 20.6 in fourths, 18.9 in sixths, 24.2 in sevenths; 16 of 4000 visible ones: 18.4 in thirds, 16.4 in

@@ -182,6 +182,8 @@ S2K_API s2k_status s2k_kv8_attend(const s2k_kv8 *c, int32_t layer, const s2k_kv8
     return launched(launch_kv8_attend(cache, rows, a, (cudaStream_t)stream), "s2k_kv8_attend");
 }
 
+S2K_API int32_t s2k_debug_kv8_attend_kernel(void) { return g_kv8_attend_kernel; }
+
 S2K_API s2k_status s2k_logprobs(int32_t device, const void *logits, int32_t type, int32_t rows, int32_t n,
                                 int64_t row_stride, const int32_t *targets, int32_t n_top, float *logprob,
                                 float *entropy, int32_t *top_ids, float *top_logprobs, void *stream) {

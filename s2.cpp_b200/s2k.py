@@ -49,7 +49,7 @@ EXPORTED = [
     "s2k_codec_stream_create", "s2k_codec_stream_free", "s2k_codec_stream_push", "s2k_codec_stream_finish",
     "s2k_codec_stream_max_release",
     "s2k_seq_create_kv8", "s2k_eval_logprobs",
-    "s2k_kv8_append", "s2k_kv8_read", "s2k_kv8_attend", "s2k_logprobs",
+    "s2k_kv8_append", "s2k_kv8_read", "s2k_kv8_attend", "s2k_logprobs", "s2k_debug_kv8_attend_kernel",
 ]
 
 REQ_WAITING, REQ_LIVE, REQ_DONE, REQ_FAILED, REQ_CANCELLED = 0, 1, 2, 3, 4  # S2K_REQ_*
@@ -253,6 +253,7 @@ def lib() -> ctypes.CDLL:
         "s2k_kv8_append": ([vp, i32, vp, vp, vp, vp], i32),
         "s2k_kv8_read": ([vp, i32, vp, vp, vp, vp], i32),
         "s2k_kv8_attend": ([vp, i32, vp, vp, vp, i32, ctypes.c_float, i32, i32, vp], i32),
+        "s2k_debug_kv8_attend_kernel": ([], i32),
         "s2k_logprobs": ([i32, vp, i32, i32, i32, ctypes.c_int64, vp, i32, vp, vp, vp, vp, vp], i32),
     }
     for name, (args, res) in sig.items():
