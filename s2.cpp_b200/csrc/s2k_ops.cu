@@ -191,6 +191,7 @@ S2K_API s2k_status s2k_logprobs(int32_t device, const void *logits, int32_t type
     if (!es) return fail(S2K_ERR_UNSUPPORTED, "logits of type %d (F32, F16 or BF16)", type);
     if (rows < 0 || n <= 0 || n > 1 << 30) return fail(S2K_ERR_ARG, "%d rows of %d logits", rows, n);
     if (row_stride < 0) return fail(S2K_ERR_ARG, "negative row stride");
+    if ((double)row_stride * std::max(rows - 1, 0) + n > kMaxExtent) return fail(S2K_ERR_ARG, "logits reach too far");
     if (n_top < 0 || n_top > S2K_LOGPROBS_MAX_TOP || n_top > n)
         return fail(S2K_ERR_ARG, "%d alternatives of %d logits (at most %d)", n_top, n, S2K_LOGPROBS_MAX_TOP);
     if (rows > 0 && (!logits || (logprob && !targets) || (n_top > 0 && (!top_ids || !top_logprobs))))

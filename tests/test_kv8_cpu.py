@@ -163,3 +163,13 @@ def test_numbers_beyond_32_bits_are_not_cut():
               lambda: s2k.logprobs(torch.zeros(1, 1).expand(big, 1))):
         with pytest.raises(s2k.S2KError, match="out of range"):
             f()
+
+
+@pytest.mark.skipif(s2k.device_count() > 0, reason="fake addresses: only where nothing can be launched")
+def test_logprobs_row_strides_whose_extents_pass_64_bits():
+    def lp(rows, ld):
+        return s2k.lib().s2k_logprobs(0, A, 0, rows, 100, ld, A, 4, A, A, A, A, None)
+    for rows, ld in ((9, 1 << 62), (2, 1 << 60), (1 << 30, 1 << 34), (3, 1 << 40)):
+        assert lp(rows, ld) == ARG, (rows, ld)
+    assert lp(1, 1 << 62) == NO_DEVICE  # one row: its stride leads nowhere
+    assert lp(9, 1 << 30) == lp(1 << 20, 155648) == lp(9, 0) == NO_DEVICE
