@@ -79,7 +79,7 @@ s2k_status check_rows(const s2k_kv8_rows *r, Kv8Rows *out) {
     // positions are int32; a grid's x dimension holds every (sequence, 16 rows)
     if (r->table_ld <= 0 || r->table_ld > INT_MAX / kPage)
         return fail(S2K_ERR_ARG, "block table of %d entries per sequence", r->table_ld);
-    if ((int64_t)r->n_seqs * (r->max_rows + 2) > INT_MAX)
+    if ((int64_t)r->n_seqs * ((int64_t)r->max_rows + 2) > INT_MAX || r->max_rows >= INT_MAX - kPage)
         return fail(S2K_ERR_ARG, "%d sequences of up to %d rows in one call", r->n_seqs, r->max_rows);
     if (r->n_seqs > 0 && (!r->past || !r->block_table)) return fail(S2K_ERR_ARG, "NULL past or block table");
     out->n_seqs = r->n_seqs;

@@ -173,3 +173,13 @@ def test_logprobs_row_strides_whose_extents_pass_64_bits():
         assert lp(rows, ld) == ARG, (rows, ld)
     assert lp(1, 1 << 62) == NO_DEVICE  # one row: its stride leads nowhere
     assert lp(9, 1 << 30) == lp(1 << 20, 155648) == lp(9, 0) == NO_DEVICE
+
+
+@pytest.mark.skipif(s2k.device_count() > 0, reason="fake addresses: only where nothing can be launched")
+def test_row_counts_next_to_32_bits():
+    """Sums of the largest row counts with a page's size must not wrap."""
+    for n in ((1 << 31) - 1, (1 << 31) - 3, (1 << 31) - 16):
+        r = rows(n_seqs=1, n_rows=n, max_rows=n)
+        assert call(r=r) == call(r=r, fn="s2k_kv8_read") == attend(r=r) == ARG, n
+    r = rows(n_seqs=1, n_rows=1 << 30, max_rows=1 << 30)
+    assert call(r=r) == NO_DEVICE
