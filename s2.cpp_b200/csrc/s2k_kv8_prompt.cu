@@ -72,7 +72,7 @@ struct PromptSmem {
     float join[2][kPM];
     float4 stat[kPMeta][kPM];  // f32 rows: a step's reference, sum and what an O of 1 is worth
     uint64_t kfull[2], kempty[2], vfull[2], vempty[2], mfull[kPMeta], sfull[2], pfull[2][2], odone[2];
-    uint64_t tfull[kPMeta], ofree[2], qfull;
+    uint64_t tfull[kPMeta], ofree[2], qfull, drained;
     uint32_t tmem;
 };
 
@@ -187,6 +187,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             mbar_init(&sm.ofree[i], 2 * kPM);
         }
         mbar_init(&sm.qfull, 8);
+        mbar_init(&sm.drained, 1);
         for (int i = 0; i < kPMeta; ++i) {
             mbar_init(&sm.mfull[i], 4);
             mbar_init(&sm.tfull[i], kPM);
@@ -353,6 +354,12 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 if (split || w) mma_commit(&sm.vempty[s]);
                 if (wide || g + 2 >= jobs) mma_commit(&sm.odone[w]);
                 if (g + 2 < jobs) ok = qk(g + 2);
+            }
+            if (!ok) {
+                // a wait ran out: the products that were issued end before the CTA gives its memory back (they wait for
+                // nothing, so this takes them microseconds)
+                mma_commit(&sm.drained);
+                mbar_wait(&sm.drained, 0, nullptr, ERR_WAIT_FULL);
             }
         }
     } else {
