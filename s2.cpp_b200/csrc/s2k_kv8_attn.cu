@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kDThreads, 3)
             top = __reduce_max_sync(kAll, top);
             // the row's largest element becomes `unit`; rows below 2^-90 as if they had one of that size
             const float amax = fmaxf(__uint_as_float(top), 8.0779356694631609e-28f);
-            const float up = __fdividef(Dg::unit, amax);
+            const float up = __fdiv_rn(Dg::unit, amax);  // __fdividef's quotient by more than 2^126 is 0
             if (lane == 0) sm.qmul[sl] = top >= 0x7f800000u ? NAN : a.scale * 1.44269504f * __fdiv_rn(1.f, up);
             uint32_t v[4] = {}, w[4];
 #pragma unroll

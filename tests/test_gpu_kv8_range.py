@@ -1,0 +1,85 @@
+"""GPU: attention over the 8-bit KV cache where queries and value scales are far from 1 or from one another, in both
+of its kernels (which one a call took is asserted).
+
+Tolerances, per row with weights w_j, largest weight w, keys k, values v, T the largest value that a key's block can
+hold (127 * its scale), n keys in view:
+  scores   e = 2^-20 * scale * sum |q k| (sums in f32 or exacter) + 2^-30 * scale * max|q| * sum |k| (a query's
+           elements are held to 2^-30 of its largest or exacter).  Each moves a weight by twice that, relative.
+  weights  their exponentials and sums 2^-18.  Few rows: fixed point relative to the largest weight * scale of a pair
+           of pages, to 2^-16 of it for 16-bit rows, 2^-30 for f32 ones: 32 keys a pair, 2 * 32 * (a page's largest
+           w_j T_j) summed over pages bounds it for either pairing.  Many rows: f16 (2^-11, twice: numerator and sum),
+           or for f32 rows f16 and what that left over; the largest w_j T_j of a row is at 2^7 or above, so f16's
+           subnormal step is worth 2^-31 of it, for each of n keys.
+  zeros    weights below 2^-126 of the largest are zero.
+  result   its type's half step, and the type's smallest number.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import kv8_util as ku
+import s2k
+from test_gpu_kv8 import DT, GRAIN, HALF_STEP, Call
+
+pytestmark = pytest.mark.gpu
+
+FEW, MANY = 1, 2
+LEAST = {"f32": 2.0**-149, "f16": 2.0**-24, "bf16": 2.0**-133}
+# a few rows; and enough for the other kernel, the last 104 of a 256-row tile's (row, head) pairs among them
+ROWS = {FEW: 2, MANY: 730}
+PAST, H, HKV = 70, 8, 2
+
+
+def make(kernel, typ, D, seed):
+    return Call([ROWS[kernel]], [PAST], H, HKV, D, typ, seed=seed)
+
+
+def check(c, kernel, q, **kw):
+    """attend, and its result for some rows against 64 bits."""
+    c.upload()
+    out = c.cache.attend(c.layer, q, *c.args, **kw)
+    assert s2k.lib().s2k_debug_kv8_attend_kernel() == kernel
+    T, scale = ROWS[kernel], c.D ** -0.5
+    k = ku.values(c.kq, c.ks, c.layer, c.table[0], PAST + T, False)
+    v = ku.values(c.vq, c.vs, c.layer, c.table[0], PAST + T, True)
+    top = np.repeat(c.vs[c.table[0, : (PAST + T + 15) // 16], c.layer].astype(np.float64), 16, 0) * 127
+    qn, on = q.double().cpu().numpy(), out.double().cpu().numpy()
+    assert np.isfinite(on).all()
+    worst = 0.0
+    for i in sorted({0, T - 1} | set(range(5, T, 61))):
+        n = PAST + i + 1
+        for h in range(H):
+            kk, vv, t, x = k[:n, h // (H // HKV)], v[:n, h // (H // HKV)], top[:, h // (H // HKV)], qn[i, h]
+            s = kk @ x * scale
+            e = scale * (2.0**-20 * (np.abs(kk) @ np.abs(x)).max() + 2.0**-30 * np.abs(x).max() * np.abs(kk).sum(1).max())
+            w = np.exp(s - s.max())
+            w /= w.sum()
+            want, mag = w @ vv, w @ np.abs(vv)
+            wt = np.zeros(len(t))
+            wt[:n] = w * t[:n]
+            if kernel == FEW:
+                tol = GRAIN[c.typ] * 64 * wt.reshape(-1, 16).max(1).sum() + mag * (2 * e + 2.0**-18)
+            else:
+                tol = 2.0**-31 * n * wt.max() + mag * (2 * e + 2.0**-18 + (0 if c.typ == "f32" else 2 * 2.0**-11))
+            tol = tol + n * 2.0**-126 * w.max() * t[:n].max() + np.abs(want) * HALF_STEP[c.typ] * 1.01 + LEAST[c.typ]
+            worst = max(worst, (np.abs(on[i, h] - want) / tol).max())
+    assert worst <= 1, f"{worst} times the tolerance"
+    return out
+
+
+KERNELS = pytest.mark.parametrize("kernel", [FEW, MANY])
+
+
+@pytest.mark.parametrize("kernel", [FEW])
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_queries_up_to_the_largest_number(D, typ, kernel):
+    """Elements around 5e37 and up to 3.3e38, keys so small that the scores are of a usual size."""
+    c = make(kernel, typ, D, 1)
+    c.ks = (c.ks / 0.01 * 1e-39).astype(np.float32)
+    q = c.rng.standard_normal((c.n, H, D)) * 5e37
+    q[:, ::3, 7] = 3.3e38 * np.sign(q[:, ::3, 7])
+    q[:, 1] *= 1e-3  # a head of smaller ones beside them
+    check(c, kernel, torch.from_numpy(np.clip(q, -3.3e38, 3.3e38)).to(DT[typ]).cuda())
