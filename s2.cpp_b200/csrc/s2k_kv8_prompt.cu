@@ -21,8 +21,8 @@
 // up to 128 slots, and f32 rows: both groups have the same 128 slots and take
 // alternate steps.
 //
-// Rounding, f16 / bf16 rows.  Q is used as it is, with K in its type (int8 is
-// exact in bf16 too).  P is f16, relative to a reference within 2^8 of the
+// Rounding, f16 / bf16 rows.  Q is used as it is, with K in its type (int8,
+// and int8 times a power of two, are exact in bf16 too).  P is f16, relative to a reference within 2^8 of the
 // running maximum, times the blocks' value scales relative to a power of two
 // above the largest seen: 2^15 at most, f16's full precision down to 2^-29 of
 // that.  O stays in TMEM (f32) and is rescaled only when a reference moves: in a
@@ -121,12 +121,15 @@ __device__ __forceinline__ void cvt_i8x4(uint32_t w, uint32_t &a, uint32_t &b) {
     a = *reinterpret_cast<const uint32_t *>(&l);
     b = *reinterpret_cast<const uint32_t *>(&h);
 }
-// The same to bf16: with m = q mod 128, 128 + m has all its bits in bf16, and q is that less 128, or less 256 where q is
-// negative: 128 with q's sign bit as its lowest exponent bit.
+// The same to bf16, times 2^-16: 128 products with the largest bf16 then stay within f32 (as they are, queries from 2.7e36
+// on gave infinite scores).  With m = q mod 128, 128 + m has all its bits in bf16, and q is that less 128, or less 256 where
+// q is negative: 128 with q's sign bit as its lowest exponent bit.
+constexpr float kBf16Keys = 65536.f;
 __device__ __forceinline__ void cvt_i8x4_bf16(uint32_t w, uint32_t &a, uint32_t &b) {
     const uint32_t m = w & 0x7f7f7f7fu, n = w & 0x80808080u;
-    uint32_t x[4] = {__byte_perm(m, 0x43434343u, 0x4140), __byte_perm(n, 0x43434343u, 0x4140),
-                     __byte_perm(m, 0x43434343u, 0x4342), __byte_perm(n, 0x43434343u, 0x4342)};
+    // 0x3b00 is 128 * 2^-16
+    uint32_t x[4] = {__byte_perm(m, 0x3b3b3b3bu, 0x4140), __byte_perm(n, 0x3b3b3b3bu, 0x4140),
+                     __byte_perm(m, 0x3b3b3b3bu, 0x4342), __byte_perm(n, 0x3b3b3b3bu, 0x4342)};
     const __nv_bfloat162 l = __hsub2(*reinterpret_cast<__nv_bfloat162 *>(&x[0]), *reinterpret_cast<__nv_bfloat162 *>(&x[1]));
     const __nv_bfloat162 h = __hsub2(*reinterpret_cast<__nv_bfloat162 *>(&x[2]), *reinterpret_cast<__nv_bfloat162 *>(&x[3]));
     a = *reinterpret_cast<const uint32_t *>(&l);
@@ -441,7 +444,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
         const int s_lo = slot0 + min(ls - lane, nslots - 1), s_hi = slot0 + min(ls - lane + 31, nslots - 1);
         const int p_min = past + row_of(s_lo), p_max = past + row_of(s_hi);
         const int wlo_row = a.window ? max(pos - a.window + 1, 0) : 0;  // the first position in the row's window
-        const float smul = wide ? sm.qmul[row] : a.scale * 1.44269504f;
+        const float smul = wide ? sm.qmul[row] : a.scale * 1.44269504f * (TYPE == OT_BF16 ? kBf16Keys : 1.f);
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t S = tmem + lanes + w * kPM, O = tmem + lanes + 2 * kPM + w * kPM;
         float ref = -INFINITY, l = 0.f, vref = 7.8886090522101181e-31f;

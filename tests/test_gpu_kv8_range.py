@@ -72,7 +72,7 @@ def check(c, kernel, q, **kw):
 KERNELS = pytest.mark.parametrize("kernel", [FEW, MANY])
 
 
-@pytest.mark.parametrize("kernel", [FEW])
+@KERNELS
 @pytest.mark.parametrize("typ", ["f32", "bf16"])
 @pytest.mark.parametrize("D", [64, 128])
 def test_queries_up_to_the_largest_number(D, typ, kernel):
