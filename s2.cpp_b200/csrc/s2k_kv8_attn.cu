@@ -15,9 +15,12 @@
 // base 256, each a row of the left operand of mma.sync m16n8k32.
 //   S = Q K^T  rows: the digits of the slots' queries, columns: keys
 //   O = P V    rows: the digits of the slots' weights, columns: dimensions
-// 16 rows are 4 slots of 4 digits for f32 rows (30 bits: f32's accuracy) or 8
-// slots of 2 digits for f16 and bf16 (15 bits of the row's largest element and
-// of the largest weight).  Keys and values go from shared memory into the
+// 16 rows are 4 slots of 4 digits (30 bits: f32's accuracy), or for f16 and bf16
+// rows of which there are more 8 slots of 2 digits: weights have 15 bits of the
+// largest one, queries 30 bits of the row's largest element in two products (a
+// few large dimensions must not cost the others their bits; with one product a
+// score was off by up to 2^-16 * max|q| * sum |k|, and 8 slots took 7 to 12 %
+// less time).  Keys and values go from shared memory into the
 // products as they are, and the integer sums are exact.  The same kernel with
 // f16 products (int8 -> f16, halves of q and p) took 573 instructions per page
 // and warp, this one ~220; mma.sync does int8 at twice the rate of f16 (both 2
@@ -79,22 +82,28 @@ constexpr float kMagic = 12582912.f;
 constexpr int kMagicBits = 0x4b400000;
 
 // How the 16 rows of a product are shared out.  Rows i and i + 8 are the upper
-// and lower digit of one 16-bit integer.  f32: rows i < 4 hold the high part h
-// and rows i >= 4 the low part of x = h * 2^15 + low, |h| <= 32512, |low| <=
-// 2^14, of slot i % 4.  16-bit types: x = h, of slot i.
-template <int TYPE>
+// and lower digit of one 16-bit integer.  4 slots (wide): rows i < 4 hold the
+// high part h and rows i >= 4 the low part of x = h * 2^15 + low, |h| <= 32512,
+// |low| <= 2^14, of slot i % 4.  8 slots: a row per slot i, weights x = h; the
+// queries' low parts are in a second product.
+constexpr float kHigh = 32768.f;  // what an upper part's unit is worth
+// the largest integers written: digits in [-128, 127] reach 127 * 257
+constexpr float kQUnit = 32512.f * kHigh;
+constexpr float kQOne = 1073741824.f;  // 2^30, what the products with queries are divided by
+// the upper or the lower part of round(x), |x| <= kQUnit, in the low 16 bits
+__device__ __forceinline__ uint32_t split_part(float x, bool low) {
+    const float h = fmaf(x, 1.f / kHigh, kMagic);
+    return __float_as_uint(low ? fmaf(h - kMagic, -kHigh, x) + kMagic : h);
+}
+template <int SLOTS>
 struct Digits {
-    static constexpr bool wide = TYPE == OT_F32;
-    static constexpr int slots = wide ? 4 : 8;
-    // the largest integer written: digits in [-128, 127] reach 127 * 257
-    static constexpr float unit = wide ? 32512.f * 32768.f : 32512.f;
-    static constexpr float high = 32768.f;  // wide: what an upper part's unit is worth
+    static constexpr bool wide = SLOTS == 4;
+    static constexpr int slots = SLOTS;
+    static constexpr float unit = wide ? 32512.f * kHigh : 32512.f;  // of the weights
     static __device__ __forceinline__ int slot(int i) { return i % slots; }
-    // the lane's part of round(x), in the low 16 bits
+    // the lane's part of round(x), a weight's, in the low 16 bits
     static __device__ __forceinline__ uint32_t part(float x, bool low) {
-        if (!wide) return __float_as_uint(x + kMagic);
-        const float h = fmaf(x, 1.f / high, kMagic);
-        return __float_as_uint(low ? fmaf(h - kMagic, -high, x) + kMagic : h);
+        return wide ? split_part(x, low) : __float_as_uint(x + kMagic);
     }
     // Four parts -> the words of their upper and lower digits.  The digits of
     // n are the bytes of n + 0x8080, less 128 each.
@@ -113,7 +122,7 @@ struct DecodeSmem {
         alignas(128) int8_t ring[kDWarps][kDStages<HD>][2][2][kPage * HD];  // page of the pair, keys / values
         float o[kDWarps][SLOTS][kRow];                                      // after the loop: each warp's output
     };
-    uint32_t q[SLOTS][SLOTS == 4 ? 4 : 2][HD / 4 + 4];  // digit words of the queries, upper first
+    uint32_t q[SLOTS][4][HD / 4 + 4];  // digit words of the queries, upper first
     float qmul[SLOTS];
     float m[kDWarps][SLOTS], l[kDWarps][SLOTS];
     // what the cluster's CTAs send: their outputs for this CTA's share, and (maximum, sum)
@@ -129,12 +138,12 @@ __device__ __forceinline__ int key_at(int x) {
     return HD == 128 ? x ^ ((x & 128) >> 1) : x;
 }
 
-template <int HD, int TYPE>
+template <int HD, int TYPE, int SLOTS>
 __global__ void __launch_bounds__(kDThreads, 3)
     kv8_decode_kernel(Kv8 c, Kv8Rows r, Kv8Attn a, int cs, float inv_group, int vec) {
     using T = typename OType<TYPE>::T;
-    using Dg = Digits<TYPE>;
-    constexpr int SLOTS = Dg::slots, STAGES = kDStages<HD>;
+    using Dg = Digits<SLOTS>;
+    constexpr int STAGES = kDStages<HD>;
     constexpr int KV = HD / 32;  // k steps of Q K^T
     constexpr int NU = HD / 8;   // column tiles of P V
     constexpr unsigned kAll = 0xffffffffu;
@@ -214,19 +223,21 @@ __global__ void __launch_bounds__(kDThreads, 3)
 #pragma unroll
             for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
             top = __reduce_max_sync(kAll, top);
-            // the row's largest element becomes `unit`; rows below 2^-90 as if they had one of that size
-            const float amax = fmaxf(__uint_as_float(top), 8.0779356694631609e-28f);
-            const float up = __fdiv_rn(Dg::unit, amax);  // __fdividef's quotient by more than 2^126 is 0
-            if (lane == 0) sm.qmul[sl] = top >= 0x7f800000u ? NAN : a.scale * 1.44269504f * __fdiv_rn(1.f, up);
+            // the row's largest element becomes kQUnit; far down, both sides by 2^64, exactly, so that the factor is finite
+            const float pre = top < 0x20000000u ? 18446744073709551616.f : 1.f;  // below 2^-63
+            const float amax = __uint_as_float(top);
+            const float up = __fdiv_rn(kQUnit, fmaxf(amax * pre, 8.0779356694631609e-28f));  // a row of zeros: 2^-90
+            // takes the scores, in units of 2^30, to base-2 logarithms
+            if (lane == 0) sm.qmul[sl] = top >= 0x7f800000u ? NAN : a.scale * 1.44269504f * (amax * (kQOne / kQUnit));
             uint32_t v[4] = {}, w[4];
 #pragma unroll
-            for (int h = 0; h < (Dg::wide ? 2 : 1); ++h) {
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = Dg::part(x[e] * up, h);
+                for (int e = 0; e < E; ++e) v[e] = split_part(x[e] * pre * up, h);
                 Dg::words(v, w[2 * h], w[2 * h + 1]);
             }
 #pragma unroll
-            for (int d = 0; d < (Dg::wide ? 4 : 2); ++d) {
+            for (int d = 0; d < 4; ++d) {
                 if (E == 4) sm.q[sl][d][lane] = w[d];
                 else reinterpret_cast<uint16_t *>(sm.q[sl][d])[lane] = (uint16_t)w[d];
             }
@@ -234,17 +245,23 @@ __global__ void __launch_bounds__(kDThreads, 3)
     }
     __syncthreads();
     uint32_t q[KV][4];
-    const float smul = sm.qmul[ls];  // takes the scores to base-2 logarithms
+    const float smul = sm.qmul[ls];
+    // the queries' digits d0 and d0 + 1 as k steps' left operands
+    auto load_q = [&](uint32_t (&t)[KV][4], int d0) {
 #pragma unroll
-    for (int j = 0; j < KV / 2; ++j)
+        for (int j = 0; j < KV / 2; ++j)
 #pragma unroll
-        for (int d = 0; d < 2; ++d) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(&sm.q[ls][(Dg::wide && li >= 4 ? 2 : 0) + d][16 * j + 4 * lc]);
-            q[2 * j][d] = w.x;
-            q[2 * j][2 + d] = w.y;
-            q[2 * j + 1][d] = w.z;
-            q[2 * j + 1][2 + d] = w.w;
-        }
+            for (int d = 0; d < 2; ++d) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(&sm.q[ls][d0 + d][16 * j + 4 * lc]);
+                t[2 * j][d] = w.x;
+                t[2 * j][2 + d] = w.y;
+                t[2 * j + 1][d] = w.z;
+                t[2 * j + 1][2 + d] = w.w;
+            }
+    };
+    load_q(q, Dg::wide && li >= 4 ? 2 : 0);
+    uint32_t q2[KV][4];
+    if (!Dg::wide) load_q(q2, 2);
     float m = -INFINITY, l = 0.f;  // l: this lane's tokens only
     float o[NU][2];
 #pragma unroll
@@ -280,7 +297,7 @@ __global__ void __launch_bounds__(kDThreads, 3)
             p0[e] = __shfl_sync(kAll, p0s, from + e);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                int acc[4];
+                int acc[4], low[4];
                 const int tok = 4 * (li >> 1) + 2 * t + (li & 1);
 #pragma unroll
                 for (int j = 0; j < KV / 2; ++j) {
@@ -288,13 +305,24 @@ __global__ void __launch_bounds__(kDThreads, 3)
                     if (j == 0) imma0(acc, q[0], w.x, w.y);
                     else imma(acc, q[2 * j], w.x, w.y);
                     imma(acc, q[2 * j + 1], w.z, w.w);
+                    if (!Dg::wide) {
+                        if (j == 0) imma0(low, q2[0], w.x, w.y);
+                        else imma(low, q2[2 * j], w.x, w.y);
+                        imma(low, q2[2 * j + 1], w.z, w.w);
+                    }
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float y = fmaf(__int_as_float(acc[h]) - kMagic, 256.f, __int_as_float(acc[2 + h]) - kMagic);
+                    // digit by digit, the result in units of 2^30
+                    auto two = [](int hi, int lo) {
+                        return fmaf(__int_as_float(hi) - kMagic, 256.f / kQOne, fmaf(__int_as_float(lo), 1.f / kQOne, -kMagic / kQOne));
+                    };
+                    float y = two(acc[h], acc[2 + h]);
                     if (Dg::wide) {
                         const float other = __shfl_xor_sync(kAll, y, 16);
-                        y = li < 4 ? fmaf(y, Dg::high, other) : fmaf(other, Dg::high, y);
+                        y = li < 4 ? fmaf(y, kHigh, other) : fmaf(other, kHigh, y);
+                    } else {
+                        y = fmaf(y, kHigh, two(low[h], low[2 + h]));
                     }
                     x[4 * e + 2 * t + h] = y * pks;
                 }
@@ -349,7 +377,7 @@ __global__ void __launch_bounds__(kDThreads, 3)
             for (int t = 0; t < 4; ++t) v[t] = Dg::part(p[4 * e + t] * g, li >= 4);
             Dg::words(v, pa[2 * e], pa[2 * e + 1]);
         }
-        const float mul = Dg::wide && li < 4 ? down * Dg::high : down;
+        const float mul = Dg::wide && li < 4 ? down * kHigh : down;
         const int8_t *v0 = sm.ring[warp][s][0][1] + lane * 4, *v1 = sm.ring[warp][s][1][1] + lane * 4;
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
@@ -453,19 +481,21 @@ static DecodeDevice g_decode[64];
 
 thread_local int g_kv8_attend_kernel = 0;
 
-template <int HD, int TYPE>
+template <int HD, int SLOTS>
 static constexpr int decode_smem() {
-    return (int)sizeof(DecodeSmem<HD, Digits<TYPE>::slots>) + 128;
+    constexpr int n = (int)sizeof(DecodeSmem<HD, SLOTS>) + 128;
+    static_assert(3 * (n + 1024) <= 228 * 1024, "three CTAs per SM");
+    return n;
 }
 
-template <int HD, int TYPE>
+template <int HD, int TYPE, int SLOTS>
 static cudaError_t decode_setup() {
-    const auto f = kv8_decode_kernel<HD, TYPE>;
-    cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, decode_smem<HD, TYPE>());
+    const auto f = kv8_decode_kernel<HD, TYPE, SLOTS>;
+    cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, decode_smem<HD, SLOTS>());
     return e != cudaSuccess ? e : cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
 }
 
-template <int HD, int TYPE>
+template <int HD, int TYPE, int SLOTS>
 static cudaError_t decode_launch(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, int cs, int tiles,
                                  cudaStream_t st) {
     cudaLaunchAttribute attr[1];
@@ -475,13 +505,13 @@ static cudaError_t decode_launch(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)r.n_seqs * cs, c.n_kv_heads, tiles);
     cfg.blockDim = dim3(kDThreads);
-    cfg.dynamicSmemBytes = decode_smem<HD, TYPE>();
+    cfg.dynamicSmemBytes = decode_smem<HD, SLOTS>();
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = cs > 1 ? 1 : 0;
     const float inv_group = 1.0f / (float)(a.n_heads / c.n_kv_heads);
     const int vec = rows_vec(a.q, 4) && rows_vec(a.out, 4);
-    return cudaLaunchKernelEx(&cfg, kv8_decode_kernel<HD, TYPE>, c, r, a, cs, inv_group, vec);
+    return cudaLaunchKernelEx(&cfg, kv8_decode_kernel<HD, TYPE, SLOTS>, c, r, a, cs, inv_group, vec);
 }
 
 cudaError_t launch_kv8_attend(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, cudaStream_t st) {
@@ -498,7 +528,13 @@ cudaError_t launch_kv8_attend(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, 
         if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev))) return e;
         for (int hd : {64, 128})
             for (int type : {OT_F32, OT_F16, OT_BF16})
-                if ((e = kv8_dispatch(hd, type, [&](auto h, auto t) { return decode_setup<h, t>(); }))) return e;
+                if ((e = kv8_dispatch(hd, type, [&](auto h, auto t) {
+                         cudaError_t e4 = decode_setup<h, t, 4>();
+                         if constexpr (t != OT_F32)
+                             if (e4 == cudaSuccess) e4 = decode_setup<h, t, 8>();
+                         return e4;
+                     })))
+                    return e;
         d.sms = sms;
         d.ready.store(1, std::memory_order_release);
     }
@@ -509,7 +545,10 @@ cudaError_t launch_kv8_attend(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, 
         const long long seen = a.window ? ((long long)a.window + rows + a.sinks) / kPage + 3 : r.table_ld;
         return std::min<long long>(seen, r.table_ld);
     };
-    const long long slots = a.q.type == OT_F32 ? Digits<OT_F32>::slots : Digits<OT_F16>::slots;
+    // 16-bit rows: 8 slots a tile, but 4 where no sequence has more, with one product in place of two (4 query heads a kv
+    // head: 64 bf16 sequences of up to 2523 tokens 43.2 us in fours, 46.5 in eights; one f16 of 32768 25.0 and 28.6)
+    const bool four = a.q.type == OT_F32 || (long long)r.max_rows * G <= 4;
+    const long long slots = four ? 4 : 8;
     const long long tiles = tiles_of(slots), pages = pages_of(slots);
     const long long groups = (long long)c.n_kv_heads * r.n_seqs, units = tiles * groups;
     // Which kernel.  Here every tile of 4 or 8 slots walks the pages, spread over the SMs: a page of a tile is the unit
@@ -536,7 +575,9 @@ cudaError_t launch_kv8_attend(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, 
     if ((long long)r.n_seqs * cs > 0x7fffffffLL) return cudaErrorInvalidValue;
     count_launch();
     return kv8_dispatch(c.head_dim, a.q.type, [&](auto hd, auto type) {
-        return decode_launch<hd, type>(c, r, a, cs, (int)tiles, st);
+        if constexpr (type != OT_F32)
+            if (!four) return decode_launch<hd, type, 8>(c, r, a, cs, (int)tiles, st);
+        return decode_launch<hd, type, 4>(c, r, a, cs, (int)tiles, st);
     });
 }
 

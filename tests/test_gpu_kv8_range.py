@@ -83,3 +83,26 @@ def test_queries_up_to_the_largest_number(D, typ, kernel):
     q[:, ::3, 7] = 3.3e38 * np.sign(q[:, ::3, 7])
     q[:, 1] *= 1e-3  # a head of smaller ones beside them
     check(c, kernel, torch.from_numpy(np.clip(q, -3.3e38, 3.3e38)).to(DT[typ]).cuda())
+
+
+@KERNELS
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+@pytest.mark.parametrize("outlier", [300.0, 3000.0])
+def test_one_large_query_element(outlier, typ, kernel):
+    """A dimension that no key uses must not cost the others their bits."""
+    c = make(kernel, typ, 128, 2)
+    c.kq[..., 5] = 0
+    q = c.heads(H, 1.5)
+    q[:, :, 5] = outlier
+    check(c, kernel, q)
+
+
+@KERNELS
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [1e-30, 1e-18])
+def test_small_queries(size, typ, kernel):
+    """Under keys as much larger."""
+    c = make(kernel, typ, 128, 5)
+    c.ks = (c.ks / size).astype(np.float32)
+    q = c.rng.standard_normal((c.n, H, 128)) * 1.5 * size
+    check(c, kernel, torch.from_numpy(q).to(DT[typ]).cuda())
