@@ -144,6 +144,9 @@ __device__ __forceinline__ uint32_t in_cta(const void *p, uint32_t rank) {
 __device__ __forceinline__ void st_cluster(uint32_t a, float x, float y) {
     asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(x), "f"(y) : "memory");
 }
+__device__ __forceinline__ void st_cluster(uint32_t a, float x) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(x) : "memory");
+}
 __device__ __forceinline__ void st_cluster(uint32_t a, float4 v) {
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
                  : "memory");

@@ -29,7 +29,10 @@
 //
 // Weights are taken relative to the largest of two pages (32 keys) with the
 // blocks' value scales in them: digits of p * v_scale / W, W the pages' largest
-// such product.  The f32 factors (W, the running maximum) multiply the sums.
+// such product.  The f32 factors (W, the running maximum) multiply the sums,
+// which are in units of a power of two, that of the largest value scale that the
+// warp met: scales may be anything that f32 holds, and no sum passes it on the
+// way.  A product below 2^-90 of that unit has fewer bits.
 //
 // The order of dimensions within a product is free as long as both operands
 // agree.  Lane (i, c) = (lane / 4, lane % 4) takes dims 16c .. 16c+15 (and 64
@@ -62,7 +65,7 @@ constexpr int kDWarps = 4;
 constexpr int kDThreads = kDWarps * 32;
 template <int HD>
 constexpr int kDStages = HD == 128 ? 2 : 4;
-// D = A B + D, or + kMagicBits: int8 digits, int32 sums.  Not volatile: the
+// D = A B + D, or + kMagic's bits: int8 digits, int32 sums.  Not volatile: the
 // order among them is the compiler's.
 __device__ __forceinline__ void imma(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -79,7 +82,6 @@ __device__ __forceinline__ void imma0(int (&d)[4], const uint32_t (&a)[4], uint3
 // bits then are the integer: conversions run at a quarter of an addition's
 // rate and took a third of the loop.
 constexpr float kMagic = 12582912.f;
-constexpr int kMagicBits = 0x4b400000;
 
 // How the 16 rows of a product are shared out.  Rows i and i + 8 are the upper
 // and lower digit of one 16-bit integer.  4 slots (wide): rows i < 4 hold the
@@ -125,9 +127,11 @@ struct DecodeSmem {
     uint32_t q[SLOTS][4][HD / 4 + 4];  // digit words of the queries, upper first
     float qmul[SLOTS];
     float m[kDWarps][SLOTS], l[kDWarps][SLOTS];
-    // what the cluster's CTAs send: their outputs for this CTA's share, and (maximum, sum)
+    int unit[kDWarps];  // exponents of the outputs' units
+    // what the cluster's CTAs send: their outputs for this CTA's share, (maximum, sum) and unit
     float4 from[SLOTS * HD / 4 + kMaxCluster];
     float2 ml[kMaxCluster][SLOTS];
+    float un[kMaxCluster];
 };
 
 // Where byte x (16-byte aligned) of a page's keys lies in shared memory: rows
@@ -137,6 +141,10 @@ template <int HD>
 __device__ __forceinline__ int key_at(int x) {
     return HD == 128 ? x ^ ((x & 128) >> 1) : x;
 }
+
+// Powers of two by their exponents as f32 holds them (1 .. 254); 2^(a - b), a <= b, 0 from 2^-127 on.
+__device__ __forceinline__ float pow2(int e) { return __int_as_float(e << 23); }
+__device__ __forceinline__ float pow2_of(int a, int b) { return __int_as_float(max(127 + a - b, 0) << 23); }
 
 template <int HD, int TYPE, int SLOTS>
 __global__ void __launch_bounds__(kDThreads, 3)
@@ -267,6 +275,8 @@ __global__ void __launch_bounds__(kDThreads, 3)
 #pragma unroll
     for (int u = 0; u < NU; ++u) o[u][0] = o[u][1] = 0.f;
     float ks = 0.f, vs = 0.f;
+    int unit = 1;      // o is in units of 2^(unit - 127): the exponent of the largest value scale met, as f32 holds it
+    float grow = 1.f;  // and is to be multiplied by this
     for (int k = 0; k < mine; ++k) {
         if (k % 16 == 0) {
             if (k) {
@@ -293,7 +303,6 @@ __global__ void __launch_bounds__(kDThreads, 3)
         for (int e = 0; e < 2; ++e) {
             const int8_t *kp = sm.ring[warp][s][e][0];
             const float pks = __shfl_sync(kAll, ks, from + e) * smul;
-            f[e] = __shfl_sync(kAll, vs, from + e);
             p0[e] = __shfl_sync(kAll, p0s, from + e);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -328,6 +337,16 @@ __global__ void __launch_bounds__(kDThreads, 3)
                 }
             }
         }
+        if (k % 16 == 0) {
+            // the unit that these pairs' scales need, and they in it: below 2, but for the last powers (after the products:
+            // the scales are still on their way before them)
+            const int e = __float_as_int(vs) >> 23, most = max(min(__reduce_max_sync(kAll, e < 255 ? e : 0), 252), unit);
+            grow = pow2_of(unit, most);
+            unit = most;
+            vs *= pow2(254 - unit);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) f[e] = __shfl_sync(kAll, vs, from + e);
         // a page at the edge of what the slots see, or none
         const int p_lo = min(p0[0], p0[1]), p_hi = max(p0[0], p0[1]);
         if (p_hi + kPage - 1 > pos_lo || (a.window && p_lo <= pos_hi - a.window && p_hi + kPage > a.sinks)) {
@@ -351,23 +370,25 @@ __global__ void __launch_bounds__(kDThreads, 3)
         const float both = fmaxf(pm[0], pm[1]);
         const float ref = both == -INFINITY ? 0.f : both;
         const float m2 = fmaxf(m, both);
-        if (__any_sync(kAll, m2 > m)) {
+        if (__any_sync(kAll, m2 > m || grow != 1.f)) {
             const float alpha = m == m2 ? 1.f : ex2(m - m2);  // 0 for the slot's first pair
             l *= alpha;
 #pragma unroll
-            for (int u = 0; u < NU; ++u) o[u][0] *= alpha, o[u][1] *= alpha;
+            for (int u = 0; u < NU; ++u) o[u][0] *= alpha * grow, o[u][1] *= alpha * grow;
             m = m2;
+            grow = 1.f;
         }
         const float f0 = both == -INFINITY ? 0.f : ex2(ref - m2);
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) p[e] = ex2(x[e] - ref);
         l += f0 * (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
-        // weights times value scales, relative to the pair's largest; a NaN scale has to reach the sum by `down`:
-        // integers do not carry it
-        const float W = fmaxf(fmaxf(ex2(pm[0] - ref) * f[0], ex2(pm[1] - ref) * f[1]), 7.8886090522101181e-31f);
+        // weights times value scales, relative to the pair's largest; a NaN scale has to reach the sum by `down`: integers
+        // do not carry it
+        const float W = fmaxf(fmaxf(ex2(pm[0] - ref) * f[0], ex2(pm[1] - ref) * f[1]), 8.0779356694631609e-28f);  // 2^-90
         const float up = __fdividef(Dg::unit, W);
         const float down = f0 * (W * (1.f / Dg::unit)) + 0.f * (f[0] + f[1]);
+        const float mul = Dg::wide && li < 4 ? down * kHigh : down;
         uint32_t pa[4];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -377,7 +398,6 @@ __global__ void __launch_bounds__(kDThreads, 3)
             for (int t = 0; t < 4; ++t) v[t] = Dg::part(p[4 * e + t] * g, li >= 4);
             Dg::words(v, pa[2 * e], pa[2 * e + 1]);
         }
-        const float mul = Dg::wide && li < 4 ? down * kHigh : down;
         const int8_t *v0 = sm.ring[warp][s][0][1] + lane * 4, *v1 = sm.ring[warp][s][1][1] + lane * 4;
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
@@ -402,27 +422,29 @@ __global__ void __launch_bounds__(kDThreads, 3)
 
     // join the warps, in order: outputs relative to the CTA's maximum
     if (li < SLOTS && lc == 0) sm.m[warp][ls] = m;
+    if (lane == 0) sm.unit[warp] = unit;
     cp_wait<0>();
     __syncthreads();  // the maxima are there, and the ring is read
     float top = sm.m[0][ls];
+    int most = sm.unit[0];
 #pragma unroll
-    for (int w = 1; w < kDWarps; ++w) top = fmaxf(top, sm.m[w][ls]);
-    const float g = m == -INFINITY ? 0.f : ex2(m - top);
+    for (int w = 1; w < kDWarps; ++w) top = fmaxf(top, sm.m[w][ls]), most = max(most, sm.unit[w]);
+    const float g = m == -INFINITY ? 0.f : ex2(m - top), go = g * pow2_of(unit, most);
     if (li < SLOTS) {
 #pragma unroll
         for (int u = 0; u < NU; ++u)
-            *reinterpret_cast<float2 *>(&sm.o[warp][ls][8 * u + 2 * lc]) = make_float2(g * o[u][0], g * o[u][1]);
+            *reinterpret_cast<float2 *>(&sm.o[warp][ls][8 * u + 2 * lc]) = make_float2(go * o[u][0], go * o[u][1]);
         if (lc == 0) sm.l[warp][ls] = g * l;  // NaN scores leave m at -inf and l NaN: 0 * NaN is NaN
     }
     __syncthreads();
     constexpr int kItems = SLOTS * HD / 4;  // of 4 dims; with a cluster each CTA joins a share of them
     const int share = (kItems + cs - 1) / cs;
-    auto put = [&](int item, float sum, float4 v) {
+    auto put = [&](int item, float sum, float4 v, float un) {
         const int st = tile * SLOTS + item / (HD / 4);
         if (item / (HD / 4) >= nslots) return;
         const int row = row_of(st);
         const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-        const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+        const float y[4] = {v.x * inv * un, v.y * inv * un, v.z * inv * un, v.w * inv * un};
         store_n<4>(reinterpret_cast<T *>(a.out.p) + (long long)(row0 + row) * a.out.row_stride +
                        (long long)(kvh * G + st - row * G) * a.out.head_stride + item % (HD / 4) * 4,
                    vec, y);
@@ -438,7 +460,7 @@ __global__ void __launch_bounds__(kDThreads, 3)
             v = make_float4(v.x + t.x, v.y + t.y, v.z + t.z, v.w + t.w);
             sum += sm.l[w][sl];
         }
-        if (cs == 1) put(item, sum, v);
+        if (cs == 1) put(item, sum, v, pow2(most));
         else {
             const int owner = item / share;
             st_cluster(in_cta(&sm.from[rank * share + item - owner * share], owner), v);
@@ -451,24 +473,26 @@ __global__ void __launch_bounds__(kDThreads, 3)
 #pragma unroll
         for (int w = 1; w < kDWarps; ++w) mm = fmaxf(mm, sm.m[w][sl]), sum += sm.l[w][sl];
         st_cluster(in_cta(&sm.ml[rank][sl], x / SLOTS), mm, sum);
+        if (sl == 0) st_cluster(in_cta(&sm.un[rank], x / SLOTS), pow2(most));
     }
     cluster_arrive();
     cluster_wait();  // from here no CTA reaches into another's shared memory
     for (int x = tid; x < min(share, kItems - rank * share); x += kDThreads) {
         const int item = rank * share + x, sl = item / (HD / 4);
-        float mm = -INFINITY, sum = 0.f;
+        float mm = -INFINITY, sum = 0.f, un = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int k = 0; k < cs; ++k) mm = fmaxf(mm, sm.ml[k][sl].x);
+        for (int k = 0; k < cs; ++k) mm = fmaxf(mm, sm.ml[k][sl].x), un = fmaxf(un, sm.un[k]);
 #pragma unroll 4
         for (int k = 0; k < cs; ++k) {
             const float2 ml = sm.ml[k][sl];
             const float4 t = sm.from[k * share + x];
             const float gk = ml.x == -INFINITY ? 0.f : ex2(ml.x - mm);
             sum += gk * ml.y;
-            v = make_float4(v.x + gk * t.x, v.y + gk * t.y, v.z + gk * t.z, v.w + gk * t.w);
+            const float go = gk * pow2_of(__float_as_int(sm.un[k]) >> 23, __float_as_int(un) >> 23);
+            v = make_float4(v.x + go * t.x, v.y + go * t.y, v.z + go * t.z, v.w + go * t.w);
         }
-        put(item, sum, v);
+        put(item, sum, v, un);
     }
 }
 

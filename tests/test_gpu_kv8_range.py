@@ -106,3 +106,33 @@ def test_small_queries(size, typ, kernel):
     c.ks = (c.ks / size).astype(np.float32)
     q = c.rng.standard_normal((c.n, H, 128)) * 1.5 * size
     check(c, kernel, torch.from_numpy(q).to(DT[typ]).cuda())
+
+
+def spread(c, kind):
+    r = c.rng.random(c.vs.shape)
+    if kind == "tiny":
+        return 1e-30 * (0.5 + r)
+    if kind == "subnormal":
+        return 10.0 ** (-41 + 3 * r)
+    if kind == "huge":
+        return 2.6e36 * (0.3 + 0.7 * r)
+    if kind == "all":
+        return 10.0 ** (-38 + 74 * r)
+    return np.where(r < 0.5, 0.0, 0.01 * r)  # zeros
+
+
+@pytest.mark.parametrize("kernel", [FEW])
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("kind", ["tiny", "subnormal", "huge", "all", "zeros"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_value_scales(D, kind, typ, kernel):
+    c = make(kernel, typ, D, 3)
+    c.vs = spread(c, kind).astype(np.float32)
+    if kind == "zeros":  # the block of the largest scores among them
+        q = c.heads(H, 0.3)
+        c.kq[c.table[0, 2], c.layer] = 90
+        c.vs[c.table[0, 2], c.layer] = 0.0
+        q += 0.2
+    else:
+        q = c.heads(H, 1.5)
+    check(c, kernel, q)
