@@ -22,18 +22,19 @@
 // alternate steps.
 //
 // Rounding, f16 / bf16 rows.  Q is used as it is, with K in its type (int8,
-// and int8 times a power of two, are exact in bf16 too).  P is f16, relative to a reference within 2^8 of the
-// running maximum, times the blocks' value scales relative to a power of two
-// above the largest seen: 2^15 at most, f16's full precision down to 2^-29 of
-// that.  O stays in TMEM (f32) and is rescaled only when a reference moves: in a
-// row's first steps and rarely after.
+// and int8 times a power of two, are exact in bf16 too).  P is f16: a weight
+// times its block's value scale, relative to a power of two within 2^7 of the
+// row's largest such product (of the largest scale, a block of large values and
+// next to no weight cost the others their bits), 2^15 at most, with f16's full
+// precision down to 2^-20 of the largest.  O stays in TMEM (f32) and is rescaled
+// only when that reference moves: in a row's first steps and rarely after.
 //
 // f32 rows.  Q (after a power of two per slot) and P are two f16 operands each,
 // rounded and left over: twice the products for 22 bits.  Sums in TMEM lose a
 // little at every addition (they are cut, not rounded), which over a long
 // context would show in f32: each step's O is taken out and added in registers,
-// half of the dimensions by each group, with the step's own maximum and value
-// scale as its reference.
+// half of the dimensions by each group, with the step's own largest weight and
+// product as its references.
 //
 // Measured: 2 x 4096 bf16 rows, 32 / 8 heads of 128: 319 us, 613 TFLOP/s; 8191
 // f16 rows under a window of 1000, 16 / 4 heads of 64: 130 us, 256 TFLOP/s; 1024
@@ -52,9 +53,12 @@ constexpr int kPM = 128;        // slots of a group, keys of a step
 constexpr int kPPages = kPM / kPage;
 constexpr int kPThreads = 512;  // warps 5-7 only make the register shares whole groups of four warps
 constexpr int kPMeta = 4;       // steps whose scales and positions are held
-constexpr float kPTop = 128.f;  // a weight at its reference, with the largest value scale
-constexpr float kPStepTop = 16384.f;  // the same for f32 rows, whose reference is the step's maximum
-constexpr float kPSlack = 8.f;  // how far (log2) the running maximum may pass the reference
+// All log2.  A weight * value scale at its reference is 2^kPTop of P, or 2^kPStepTop for f32 rows, whose reference is the
+// step's own; how far the largest product may pass its reference, and the running maximum of the scores its own; and how
+// far the product's reference is kept above a scale in view (its factor has to be finite).
+constexpr float kPTop = 7.f, kPStepTop = 14.f, kPSlack = 7.f, kPScoreSlack = 8.f, kPBelow = 100.f;
+constexpr float kPFar = 1048576.f;  // sums of scores from here on with a scale's exponent lose bits that matter
+constexpr float kPRound = 12582912.f;  // 1.5 * 2^23: an integer added to it is in its low bits
 constexpr int kPNone = 0x7fffff00;  // "first token" of no page: behind every position
 
 template <int HD>
@@ -65,12 +69,14 @@ struct PromptSmem {
     alignas(1024) uint8_t v[2][2][HD * 128];
     float qmul[kPM];
     struct Meta {
-        float ks[kPPages], vs[kPPages];
+        // a value scale is between 2^ve and twice that; vb: its bits, but with an exponent of any size (0: far below)
+        float ks[kPPages], ve[kPPages];
+        int vb[kPPages];
         int p0[kPPages];
     };
     alignas(16) Meta meta[kPMeta];
-    float join[2][kPM];
-    float4 stat[kPMeta][kPM];  // f32 rows: a step's reference, sum and what an O of 1 is worth
+    float join[3][kPM];
+    float4 stat[kPMeta][kPM];  // f32 rows: a step's reference, sum and its products' reference
     uint64_t kfull[2], kempty[2], vfull[2], vempty[2], mfull[kPMeta], sfull[2], pfull[2][2], odone[2];
     uint64_t tfull[kPMeta], ofree[2], qfull, drained;
     uint32_t tmem;
@@ -267,7 +273,12 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             if (lane < 2) {
                 typename Sm::Meta &m = sm.meta[t % kPMeta];
                 m.ks[2 * pw + lane] = ks;
-                m.vs[2 * pw + lane] = vs;
+                // subnormal scales by way of 2^32; a block with an infinite or NaN one is NaN to whoever sees it
+                const bool sub = vs < 1.17549435e-38f, none = vs == 0.f;
+                const int bits = __float_as_int(sub ? vs * 4294967296.f : vs), e = bits >> 23 & 255;
+                if (e == 255) m.ks[2 * pw + lane] = NAN;
+                m.vb[2 * pw + lane] = none || e == 255 ? -(1 << 30) : bits - (sub ? 32 << 23 : 0);
+                m.ve[2 * pw + lane] = none || e == 255 ? -200.f : (float)(e - (sub ? 159 : 127));
                 m.p0[2 * pw + lane] = own >= 0 ? first_token(t) : kPNone;
             }
             __syncwarp();
@@ -447,13 +458,14 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
         const float smul = wide ? sm.qmul[row] : a.scale * 1.44269504f * (TYPE == OT_BF16 ? kBf16Keys : 1.f);
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t S = tmem + lanes + w * kPM, O = tmem + lanes + 2 * kPM + w * kPM;
-        float ref = -INFINITY, l = 0.f, vref = 7.8886090522101181e-31f;
+        // log2 of the weights' reference (an integer), and of the products' relative to it
+        float ref = -INFINITY, l = 0.f, vr = -INFINITY;
         // f32 rows: this group's half of the output
         constexpr int HALF = wide ? HD / 2 : 1;
         float acc[HALF];
 #pragma unroll
         for (int i = 0; i < HALF; ++i) acc[i] = 0.f;
-        float top_ref = -INFINITY, sum = 0.f;
+        float top_ref = -INFINITY, top_vr = -INFINITY, sum = 0.f;
         auto take = [&](int t) {  // f32 rows: adds step t's output
             bool fine = kv8_wait(r, &sm.tfull[t % kPMeta], (t / kPMeta) & 1, ERR_WAIT_FULL) &&
                         kv8_wait(r, &sm.odone[t & 1], (t >> 1) & 1, ERR_WAIT_FULL);
@@ -461,10 +473,12 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             tc_fence_after();
             const float4 z = sm.stat[t % kPMeta][row];
             const float r2 = fmaxf(top_ref, z.x);
-            const float f0 = top_ref == r2 ? 1.f : ex2(top_ref - r2), f1 = z.x == -INFINITY ? 0.f : ex2(z.x - r2);
-            const float mul = f1 * z.z;
-            sum = sum * f0 + z.y * f1;
+            const float d0 = top_ref == r2 ? 0.f : top_ref - r2, d1 = z.x == r2 ? 0.f : z.x - r2;
+            const float e0 = top_vr + d0, e1 = z.z + d1, v2 = fmaxf(e0, e1);
+            const float f0 = e0 == v2 ? 1.f : ex2(e0 - v2), mul = z.z == -INFINITY ? 0.f : ex2(e1 - v2 - kPStepTop);
+            sum = sum * ex2(d0) + (z.x == -INFINITY ? 0.f * z.y : z.y * ex2(d1));
             top_ref = r2;
+            top_vr = v2;
             const uint32_t from = tmem + lanes + 2 * kPM + (t & 1) * kPM + w * HALF;
 #pragma unroll
             for (int ch = 0; ch < (HALF + 15) / 16; ++ch) {
@@ -491,12 +505,12 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             tc_fence_after();
             const typename Sm::Meta &m = sm.meta[t % kPMeta];
             int lo = m.p0[0], hi = m.p0[0];
-            float vmax = m.vs[0];  // of the blocks that the row sees: its weights' resolution goes by them
+            float vl = m.ve[0];  // the largest value scale that the row sees
 #pragma unroll
             for (int i = 1; i < kPPages; ++i) {
                 lo = min(lo, m.p0[i]);
                 hi = max(hi, m.p0[i]);
-                vmax = fmaxf(vmax, m.vs[i]);
+                vl = fmaxf(vl, m.ve[i]);
             }
             const bool edge = hi + kPage - 1 > p_min || (a.window && lo <= p_max - a.window && hi + kPage > a.sinks) || a.scale < 0.f;
             // bit i: the row sees token i of page pg
@@ -505,11 +519,15 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 const int p0 = m.p0[pg];
                 return below(pos + 1 - p0) & (~below(wlo_row - p0) | below(a.sinks - p0));
             };
-            // the step's largest score.  Loops stay rolled: unrolled, with the next columns' loads ahead, they took twice
-            // as long (the instruction cache serves ten warps in five places).
-            float mx = -INFINITY;
+            // the step's largest score, and log2 of its largest product over b.  Loops stay rolled: unrolled, with the next
+            // columns' loads ahead, they took twice as long (the instruction cache serves ten warps in five places).
+            float mx = -INFINITY, us = -INFINITY, b = ref == -INFINITY ? 0.f : ref;
             uint32_t any = 0;
-            auto whole_max = [&](const int(&y)[32], float k0, float k1) {
+            auto page_max = [&](int pg, float t) {
+                mx = fmaxf(mx, t);
+                us = fmaxf(us, (t - b) + m.ve[pg]);
+            };
+            auto whole_max = [&](int ch, const int(&y)[32], float k0, float k1) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     float t0 = -INFINITY, t1 = -INFINITY;
@@ -518,53 +536,69 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                         t0 = fmaxf(fmaxf(t0, __int_as_float(y[16 * e + i])), __int_as_float(y[16 * e + i + 1]));
                         t1 = fmaxf(fmaxf(t1, __int_as_float(y[16 * e + i + 2])), __int_as_float(y[16 * e + i + 3]));
                     }
-                    mx = fmaxf(mx, fmaxf(t0, t1) * (e ? k1 : k0));
+                    page_max(2 * ch + e, fmaxf(t0, t1) * (e ? k1 : k0));
                 }
             };
-            if (!edge) {
 #pragma unroll 1
-                for (int ch = 0; ch < 4; ++ch) {
-                    int y[32];
-                    tmem_ld32(S + 32 * ch, y);
-                    whole_max(y, m.ks[2 * ch] * smul, m.ks[2 * ch + 1] * smul);
-                }
-                any = 1;
-            } else {
-                vmax = 0.f;
+            for (bool last = false;; last = true) {
+                if (!edge) {
 #pragma unroll 1
-                for (int ch = 0; ch < 4; ++ch) {
-                    int y[32];
-                    tmem_ld32(S + 32 * ch, y);
-                    const float k0 = m.ks[2 * ch] * smul, k1 = m.ks[2 * ch + 1] * smul;
-                    const uint32_t b0 = seen(2 * ch), b1 = seen(2 * ch + 1), bits = b0 | b1 << 16;
-                    any |= bits;
-                    if (b0) vmax = fmaxf(vmax, m.vs[2 * ch]);
-                    if (b1) vmax = fmaxf(vmax, m.vs[2 * ch + 1]);
-                    if (__all_sync(kAll, bits == 0)) continue;
-                    // the largest product is the largest score's unless the scale is negative
-                    if (__all_sync(kAll, bits == ~0u) && a.scale >= 0.f) {
-                        whole_max(y, k0, k1);
-                        continue;
+                    for (int ch = 0; ch < 4; ++ch) {
+                        int y[32];
+                        tmem_ld32(S + 32 * ch, y);
+                        whole_max(ch, y, m.ks[2 * ch] * smul, m.ks[2 * ch + 1] * smul);
                     }
+                    any = 1;
+                } else {
+                    vl = -INFINITY;
+#pragma unroll 1
+                    for (int ch = 0; ch < 4; ++ch) {
+                        int y[32];
+                        tmem_ld32(S + 32 * ch, y);
+                        const float k0 = m.ks[2 * ch] * smul, k1 = m.ks[2 * ch + 1] * smul;
+                        const uint32_t b0 = seen(2 * ch), b1 = seen(2 * ch + 1), bits = b0 | b1 << 16;
+                        any |= bits;
+                        if (b0) vl = fmaxf(vl, m.ve[2 * ch]);
+                        if (b1) vl = fmaxf(vl, m.ve[2 * ch + 1]);
+                        if (__all_sync(kAll, bits == 0)) continue;
+                        // the largest product is the largest score's unless the scale is negative
+                        if (__all_sync(kAll, bits == ~0u) && a.scale >= 0.f) {
+                            whole_max(ch, y, k0, k1);
+                            continue;
+                        }
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        mx = fmaxf(mx, bits >> i & 1 ? __int_as_float(y[i]) * (i < 16 ? k0 : k1) : -INFINITY);
+                        for (int e = 0; e < 2; ++e) {
+                            float t0 = -INFINITY;
+#pragma unroll
+                            for (int i = 0; i < kPage; ++i)
+                                t0 = fmaxf(t0, bits >> (16 * e + i) & 1 ? __int_as_float(y[16 * e + i]) * (e ? k1 : k0) : -INFINITY);
+                            page_max(2 * ch + e, t0);
+                        }
+                    }
                 }
+                // scores so large that they swallow a scale's exponent, unless b is next to them: once more
+                const bool large = fabsf(mx) > kPFar && mx != -INFINITY;
+                if (last || !__any_sync(kAll, large)) break;
+                if (large) b = ceilf(mx);
+                us = -INFINITY;
             }
             // keys in view and no number among their scores: an infinite or NaN query or scale
             const float odd = any && mx == -INFINITY ? NAN : 0.f;
-            // a power of two from vmax on
-            const float v2 = __uint_as_float((__float_as_uint(vmax) + 0x7fffffu) & 0x7f800000u);
+            const bool far = wide || mx > ref + kPScoreSlack;  // true for the first finite one
+            const float r2 = far ? ceilf(mx) : ref, moved = far && r2 != ref ? r2 - ref : 0.f;
+            // the products' reference that this step asks for, relative to r2
+            const float need = fmaxf(r2 == -INFINITY ? us : us - (r2 - b), vl - kPBelow);
             if (wide) {
-                ref = mx;
-                vref = fmaxf(v2, 7.8886090522101181e-31f);
+                ref = r2;
+                vr = any ? ceilf(need) : -INFINITY;
             } else {
-                const bool far = mx > ref + kPSlack;  // true for the first finite one
-                if (__any_sync(kAll, far || vmax > vref)) {
-                    const float r2 = far ? mx : ref, vn = vmax > vref ? v2 : vref;
-                    const float fl = ref == r2 ? 1.f : ex2(ref - r2), f = fl * (vref / vn);
-                    l *= fl;
-                    if (done) {
+                const float old = vr - moved;
+                const bool grow = need > old + kPSlack;
+                if (__any_sync(kAll, far || grow)) {
+                    if (far) l *= ex2(-moved);
+                    vr = grow ? ceilf(need) : old;
+                    if (done && __any_sync(kAll, grow)) {
+                        const float f = grow ? ex2(old - vr) : 1.f;
 #pragma unroll 2
                         for (int ch = 0; ch < HD / 16; ++ch) {
                             int z[16];
@@ -576,17 +610,18 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                         }
                     }
                     ref = r2;
-                    vref = vn;
                 }
             }
             const float base = ref == -INFINITY ? 0.f : ref;
-            const float vmul = (wide ? kPStepTop : kPTop) / vref;
+            // a page's scale times 2^(top - vr) by its bits; 0 where that is below every normal number
+            const int vc = __float_as_int(kPRound + (wide ? kPStepTop : kPTop) - vr) << 23;
+            auto scale_of = [&](int pg) { return __int_as_float(__viaddmax_s32(m.vb[pg], vc, 0)); };
             float l0 = odd, l1 = 0.f;
             auto weights = [&](int ch, const int(&y)[32], auto masked) {
                 uint32_t hi16[16], lo16[16];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float ks = m.ks[2 * ch + e] * smul, vs = m.vs[2 * ch + e] * vmul;
+                    const float ks = m.ks[2 * ch + e] * smul, vs = scale_of(2 * ch + e);
                     const uint32_t bits = masked ? seen(2 * ch + e) : 0;
 #pragma unroll
                     for (int i = 0; i < kPage; i += 2) {
@@ -643,7 +678,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 }
             }
             if (wide) {
-                sm.stat[t % kPMeta][row] = make_float4(ref, l0 + l1, vref * (1.f / kPStepTop), 0.f);
+                sm.stat[t % kPMeta][row] = make_float4(ref, l0 + l1, vr, 0.f);
                 mbar_arrive(&sm.tfull[t % kPMeta]);
                 if (g > 0) ok = take(g - 1);
             } else {
@@ -684,15 +719,22 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 }
             }
         };
+        // f times 2^e as f * rest: 2^e may be subnormal
+        auto in_two = [](float e, float &f, float &rest) {
+            if (e == -INFINITY) e = 0.f;
+            f *= ex2(fmaxf(e, -64.f));
+            rest = ex2(fminf(e + 64.f, 0.f));
+        };
         if (wide) {
             if (ok) ok = take(jobs - 1);
             if (!__all_sync(kAll, ok)) sum = NAN;  // a wait ran out: the result says so
-            const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+            float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum), rest;
+            in_two(top_vr, inv, rest);
 #pragma unroll
             for (int i = 0; i < HALF; i += 16) {
                 float z[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) z[e] = acc[(i + e) % HALF] * inv;
+                for (int e = 0; e < 16; ++e) z[e] = acc[(i + e) % HALF] * inv * rest;
                 lay(i, z);
             }
             store_rows(w * HALF);
@@ -702,52 +744,54 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             ok = __all_sync(kAll, ok);
             if (!ok) l = NAN;
             tc_fence_after();
-            float f = done ? vref * (1.f / kPTop) : 0.f;   // takes O to sums of weight * value
             float *xch = reinterpret_cast<float *>(sm.k);  // [kPM][HD + 4], over K and V
             if (split) {
                 if (w == 1) {
 #pragma unroll 1
                     for (int ch = 0; ch < HD / 16; ++ch) {
-                        int x[16];
+                        int x[16] = {};
                         if (done) tmem_ld16(O + 16 * ch, x);
 #pragma unroll
                         for (int i = 0; i < 16; i += 4)
-                            *reinterpret_cast<float4 *>(&xch[row * (HD + 4) + 16 * ch + i]) =
-                                done ? make_float4(__int_as_float(x[i]) * f, __int_as_float(x[i + 1]) * f,
-                                                   __int_as_float(x[i + 2]) * f, __int_as_float(x[i + 3]) * f)
-                                     : make_float4(0.f, 0.f, 0.f, 0.f);
+                            *reinterpret_cast<int4 *>(&xch[row * (HD + 4) + 16 * ch + i]) = make_int4(x[i], x[i + 1], x[i + 2], x[i + 3]);
                     }
                     sm.join[0][row] = ref;
                     sm.join[1][row] = l;
+                    sm.join[2][row] = vr;
                 }
                 named_sync(1, 2 * kPM);
             }
             if ((!split || w == 0) && ls - lane < nslots) {
-                float g1 = 0.f;
+                float f0 = 1.f, f1 = 0.f;  // the groups' outputs to the larger of their units
                 if (split) {
                     const float ref1 = sm.join[0][row], top = fmaxf(ref, ref1);
-                    const float g0 = ref == -INFINITY ? 0.f : ex2(ref - top);
-                    g1 = ref1 == -INFINITY ? 0.f : ex2(ref1 - top);
-                    l = g0 * l + g1 * sm.join[1][row];
-                    f *= g0;
+                    const float d0 = ref == top ? 0.f : ref - top, d1 = ref1 == top ? 0.f : ref1 - top;
+                    const float e0 = vr + d0, e1 = sm.join[2][row] + d1;
+                    l = (ref == -INFINITY ? 0.f * l : ex2(d0) * l) + (ref1 == -INFINITY ? 0.f * sm.join[1][row] : ex2(d1) * sm.join[1][row]);
+                    vr = fmaxf(e0, e1);
+                    f0 = e0 == vr ? 1.f : ex2(e0 - vr);
+                    f1 = e1 == vr ? 1.f : ex2(e1 - vr);
                 }
-                const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+                float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l), rest;
+                in_two(vr - kPTop, inv, rest);
+                f0 *= inv;
+                f1 *= inv;
 #pragma unroll 1
                 for (int ch = 0; ch < HD / 16; ++ch) {
                     int x[16];
                     tmem_ld16(O + 16 * ch, x);
                     float z[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) z[i] = __int_as_float(x[i]) * f;
+                    for (int i = 0; i < 16; ++i) z[i] = __int_as_float(x[i]) * f0;
                     if (split) {
 #pragma unroll
                         for (int i = 0; i < 16; i += 4) {
                             const float4 o1 = *reinterpret_cast<const float4 *>(&xch[row * (HD + 4) + 16 * ch + i]);
-                            z[i] += g1 * o1.x, z[i + 1] += g1 * o1.y, z[i + 2] += g1 * o1.z, z[i + 3] += g1 * o1.w;
+                            z[i] += f1 * o1.x, z[i + 1] += f1 * o1.y, z[i + 2] += f1 * o1.z, z[i + 3] += f1 * o1.w;
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) z[i] *= inv;
+                    for (int i = 0; i < 16; ++i) z[i] *= rest;
                     lay(16 * ch, z);
                 }
                 store_rows(0);

@@ -8,8 +8,8 @@ hold (127 * its scale), n keys in view:
   weights  their exponentials and sums 2^-18.  Few rows: fixed point relative to the largest weight * scale of a pair
            of pages, to 2^-16 of it for 16-bit rows, 2^-30 for f32 ones: 32 keys a pair, 2 * 32 * (a page's largest
            w_j T_j) summed over pages bounds it for either pairing.  Many rows: f16 (2^-11, twice: numerator and sum),
-           or for f32 rows f16 and what that left over; the largest w_j T_j of a row is at 2^7 or above, so f16's
-           subnormal step is worth 2^-31 of it, for each of n keys.
+           or for f32 rows f16 and what that left over; the largest w_j T_j of a row is at 2^6 or above, so f16's
+           subnormal step (half of 2^-24) is worth 2^-31 of it, for each of n keys.
   zeros    weights below 2^-126 of the largest are zero.
   result   its type's half step, and the type's smallest number.
 """
@@ -121,7 +121,7 @@ def spread(c, kind):
     return np.where(r < 0.5, 0.0, 0.01 * r)  # zeros
 
 
-@pytest.mark.parametrize("kernel", [FEW])
+@KERNELS
 @pytest.mark.parametrize("typ", ["f32", "bf16"])
 @pytest.mark.parametrize("kind", ["tiny", "subnormal", "huge", "all", "zeros"])
 @pytest.mark.parametrize("D", [64, 128])
@@ -136,3 +136,49 @@ def test_value_scales(D, kind, typ, kernel):
     else:
         q = c.heads(H, 1.5)
     check(c, kernel, q)
+
+
+@KERNELS
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("ratio", [1e4, 1e6, 1e8])
+def test_large_value_scales_of_small_weights(ratio, typ, kernel):
+    """Every third page has values `ratio` times the others' and scores ~20 below them: it must not cost the others'
+    weights their bits."""
+    c = make(kernel, typ, 128, 4)
+    sign = np.where(c.rng.random(128) < 0.5, -1, 1)
+    for pg in c.table[0, : (PAST + ROWS[kernel] + 15) // 16][1::3]:
+        c.kq[pg, c.layer] = (-60 * sign).astype(np.int8)
+        c.ks[pg, c.layer] = 0.01
+        c.vs[pg, c.layer] *= ratio if typ != "f16" else min(ratio, 1e6)
+    q = torch.from_numpy(c.rng.standard_normal((c.n, H, 128)) * 0.3 + 3.0 * sign).to(DT[typ]).cuda()
+    check(c, kernel, q)
+
+
+@KERNELS
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("size", [1e4])
+def test_sure_rows_beside_large_value_scales(size, typ, kernel):
+    """One key whose score is ahead by `size` and more: the result is its value, whatever the other pages hold."""
+    c = make(kernel, typ, 128, 6)
+    n = PAST + ROWS[kernel]
+    key = 21  # in the third page of 16
+    c.kq[:, c.layer] = 0
+    c.ks[:, c.layer] = 1.0
+    for pg in c.table[0, : (n + 15) // 16]:
+        c.kq[pg, c.layer, :, :, 0] = c.rng.integers(-100, 60, (HKV, 16))
+        c.vs[pg, c.layer] *= 1e6
+    at = c.table[0, key // 16]
+    c.kq[at, c.layer, :, key % 16, 0] = 127
+    c.vs[at, c.layer] /= 1e6
+    q = torch.zeros(c.n, H, 128, dtype=DT[typ], device="cuda")
+    q[:, :, 0] = size if typ != "f16" else min(size, 3e4)
+    c.upload()
+    out = c.cache.attend(c.layer, q, *c.args).double().cpu().numpy()
+    assert s2k.lib().s2k_debug_kv8_attend_kernel() == kernel
+    # the other weights are below e^-5000; the value is off by the weight's rounding in numerator and result
+    want = ku.values(c.vq, c.vs, c.layer, c.table[0], n, True)[key].repeat(H // HKV, 0)
+    step = {"f32": 2.0**-20, "f16": 2.0**-11, "bf16": 2.0**-8}[typ] + (0 if typ == "f32" else 2 * 2.0**-11)
+    top = c.vs[at, c.layer].max() * 127
+    # few rows: fixed point relative to the largest weight * scale, here the key's own
+    assert np.all(np.abs(out - want) <= step * np.abs(want) + GRAIN[typ] * top + LEAST[typ])
+
