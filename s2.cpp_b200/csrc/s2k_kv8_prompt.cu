@@ -539,6 +539,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                     page_max(2 * ch + e, fmaxf(t0, t1) * (e ? k1 : k0));
                 }
             };
+            bool careful;
 #pragma unroll 1
             for (bool last = false;; last = true) {
                 if (!edge) {
@@ -578,7 +579,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 }
                 // scores so large that they swallow a scale's exponent, unless b is next to them: once more
                 const bool large = fabsf(mx) > kPFar && mx != -INFINITY;
-                if (last || !__any_sync(kAll, large)) break;
+                careful = __any_sync(kAll, large);
+                if (last || !careful) break;
                 if (large) b = ceilf(mx);
                 us = -INFINITY;
             }
@@ -617,6 +619,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
             const int vc = __float_as_int(kPRound + (wide ? kPStepTop : kPTop) - vr) << 23;
             auto scale_of = [&](int pg) { return __int_as_float(__viaddmax_s32(m.vb[pg], vc, 0)); };
             float l0 = odd, l1 = 0.f;
+            // masked: some keys are hidden, or scores are large
             auto weights = [&](int ch, const int(&y)[32], auto masked) {
                 uint32_t hi16[16], lo16[16];
 #pragma unroll
@@ -626,7 +629,12 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
 #pragma unroll
                     for (int i = 0; i < kPage; i += 2) {
                         float p[2] = {-base, -base};
-                        fma2(p, ks, __int_as_float(y[16 * e + i]), __int_as_float(y[16 * e + i + 1]));
+                        if (masked) {  // large scores: rounded like the maximum, which they must not pass
+                            p[0] += __fmul_rn(__int_as_float(y[16 * e + i]), ks);
+                            p[1] += __fmul_rn(__int_as_float(y[16 * e + i + 1]), ks);
+                        } else {
+                            fma2(p, ks, __int_as_float(y[16 * e + i]), __int_as_float(y[16 * e + i + 1]));
+                        }
                         p[0] = ex2(p[0]);
                         p[1] = ex2(p[1]);
                         if (masked) {  // a hidden block's scales may be NaN
@@ -652,7 +660,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                 tc_fence_before();
                 mbar_arrive(&sm.pfull[w][h]);
             };
-            if (!edge) {
+            if (!edge && !careful) {
 #pragma unroll 1
                 for (int ch = 0; ch < 4; ++ch) {
                     int y[32];
@@ -671,7 +679,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                     } else {
                         int y[32];
                         tmem_ld32(S + 32 * ch, y);
-                        if (__all_sync(kAll, bits == ~0u)) weights(ch, y, std::false_type());
+                        if (__all_sync(kAll, bits == ~0u) && !careful) weights(ch, y, std::false_type());
                         else weights(ch, y, std::true_type());
                     }
                     if (ch & 1) half_done(ch / 2);

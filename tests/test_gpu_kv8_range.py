@@ -156,7 +156,7 @@ def test_large_value_scales_of_small_weights(ratio, typ, kernel):
 
 @KERNELS
 @pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("size", [1e4])
+@pytest.mark.parametrize("size", [1e4, 1e8])
 def test_sure_rows_beside_large_value_scales(size, typ, kernel):
     """One key whose score is ahead by `size` and more: the result is its value, whatever the other pages hold."""
     c = make(kernel, typ, 128, 6)
