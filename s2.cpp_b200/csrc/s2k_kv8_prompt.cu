@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                     page_max(2 * ch + e, fmaxf(t0, t1) * (e ? k1 : k0));
                 }
             };
-            bool careful;
+            bool large, careful;
 #pragma unroll 1
             for (bool last = false;; last = true) {
                 if (!edge) {
@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                     }
                 }
                 // scores so large that they swallow a scale's exponent, unless b is next to them: once more
-                const bool large = fabsf(mx) > kPFar && mx != -INFINITY;
+                large = fabsf(mx) > kPFar && fabsf(mx) < INFINITY;
                 careful = __any_sync(kAll, large);
                 if (last || !careful) break;
                 if (large) b = ceilf(mx);
@@ -614,7 +614,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                     ref = r2;
                 }
             }
-            const float base = ref == -INFINITY ? 0.f : ref;
+            // what is taken from the scores: large ones are rounded first like the maximum, which they must not pass
+            const float base = ref == -INFINITY ? 0.f : ref, fused = large ? 0.f : -base, apart = large ? -base : 0.f;
             // a page's scale times 2^(top - vr) by its bits; 0 where that is below every normal number
             const int vc = __float_as_int(kPRound + (wide ? kPStepTop : kPTop) - vr) << 23;
             auto scale_of = [&](int pg) { return __int_as_float(__viaddmax_s32(m.vb[pg], vc, 0)); };
@@ -628,13 +629,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv8_prompt_kernel(Kv8 c, Kv8Rows
                     const uint32_t bits = masked ? seen(2 * ch + e) : 0;
 #pragma unroll
                     for (int i = 0; i < kPage; i += 2) {
-                        float p[2] = {-base, -base};
-                        if (masked) {  // large scores: rounded like the maximum, which they must not pass
-                            p[0] += __fmul_rn(__int_as_float(y[16 * e + i]), ks);
-                            p[1] += __fmul_rn(__int_as_float(y[16 * e + i + 1]), ks);
-                        } else {
-                            fma2(p, ks, __int_as_float(y[16 * e + i]), __int_as_float(y[16 * e + i + 1]));
-                        }
+                        float p[2] = {fused, fused};
+                        fma2(p, ks, __int_as_float(y[16 * e + i]), __int_as_float(y[16 * e + i + 1]));
+                        if (masked) add2(p[0], p[1], apart);
                         p[0] = ex2(p[0]);
                         p[1] = ex2(p[1]);
                         if (masked) {  // a hidden block's scales may be NaN

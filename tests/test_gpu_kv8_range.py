@@ -182,3 +182,39 @@ def test_sure_rows_beside_large_value_scales(size, typ, kernel):
     # few rows: fixed point relative to the largest weight * scale, here the key's own
     assert np.all(np.abs(out - want) <= step * np.abs(want) + GRAIN[typ] * top + LEAST[typ])
 
+
+
+@KERNELS
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+def test_rows_do_not_change_with_their_neighbours(typ, kernel):
+    """A row of very large finite scores, and an infinite one, beside others: their bits stay."""
+    c = make(kernel, typ, 128, 7)
+    q = c.heads(H, 1.5)
+    want = c.cache.attend(c.layer, q, *c.args)
+    odd = q.clone()
+    odd[0, 0] *= 3e4
+    odd[0, 3] = float("inf")
+    odd[1, 2] *= -3e4
+    got = c.cache.attend(c.layer, odd, *c.args)
+    assert s2k.lib().s2k_debug_kv8_attend_kernel() == kernel
+    for r, h in ((0, 0), (0, 3), (1, 2)):  # f16 has no number for some of them
+        assert (torch.isfinite if torch.isfinite(odd[r, h]).all() else torch.isnan)(got[r, h]).all()
+        got[r, h] = want[r, h]
+    assert torch.equal(got, want)
+
+
+@KERNELS
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+def test_hidden_blocks_of_any_scale(typ, kernel):
+    """A window before which blocks hold infinities, NaN and the largest scales; behind the rows as well."""
+    T = 2 if kernel == FEW else 2400
+    c = Call([T], [PAST], H, HKV, 64, typ, seed=8)
+    q = c.heads(H, 1.5)
+    want = c.cache.attend(c.layer, q, *c.args, window=20, sinks=3)
+    keep = [int(p) for p in c.table[0, [0]]] + [int(p) for p in c.table[0, (PAST - 20) // 16:(PAST + T + 15) // 16]]
+    gone = np.setdiff1d(np.arange(c.kq.shape[0]), keep)
+    for scale in (np.inf, np.nan, 2e36):
+        c.vs[gone] = c.ks[gone] = scale
+        c.upload()
+        assert torch.equal(c.cache.attend(c.layer, q, *c.args, window=20, sinks=3), want)
+        assert s2k.lib().s2k_debug_kv8_attend_kernel() == kernel
