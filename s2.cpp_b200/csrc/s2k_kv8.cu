@@ -13,9 +13,7 @@
 // e = x - n s tells: n is right iff |e| < s/2 (or = and n is even).  One fma
 // gives e exactly: it is a multiple of s's last place (for n = 0 it is x) and
 // not larger than about s/2, so it fits 24 bits.  The stored integers are then a
-// function of the inputs alone, whatever computes them.  (Before, quotients
-// near a half were divided again in double.  16-bit inputs have one in nearly
-// every block: eight prompts of bf16 rows took 123 us, f32 ones 67.)
+// function of the inputs alone, whatever computes them.
 //
 // int8 with a block's scale rather than an 8-bit float: over a block of normal
 // values the uniform step's error is about a third of e4m3's, and every

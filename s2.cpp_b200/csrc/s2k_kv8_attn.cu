@@ -20,8 +20,8 @@
 // largest one, queries 30 bits of the row's largest element in two products (a
 // few large dimensions must not cost the others their bits; with one product a
 // score was off by up to 2^-16 * max|q| * sum |k|, and 8 slots took 7 to 12 %
-// less time).  Keys and values go from shared memory into the
-// products as they are, and the integer sums are exact.  The same kernel with
+// less time).  Keys and values go from shared memory into the products as they
+// are, and the integer sums are exact.  The same kernel with
 // f16 products (int8 -> f16, halves of q and p) took 573 instructions per page
 // and warp, this one ~220; mma.sync does int8 at twice the rate of f16 (both 2
 // cycles per instruction and SM, measured).  tcgen05 has 128 rows: 16 of them
@@ -42,10 +42,9 @@
 //
 // One warp walks its own pairs of pages through its own ring of 16-byte
 // asynchronous copies with a running maximum, sum and output; no barrier inside
-// the loop.  The pages of a (tile,
-// kv head, sequence) are split over the CTAs of a cluster when there are few
-// of them, and joined through distributed shared memory: no workspace, one
-// launch, and the same order of sums every time.
+// the loop.  The pages of a (tile, kv head, sequence) are split over the CTAs of
+// a cluster when there are few of them, and joined through distributed shared
+// memory: no workspace, one launch, and the same order of sums every time.
 #include "s2k_common.cuh"
 #include "s2k_kv8.h"
 
@@ -59,8 +58,9 @@ namespace s2k {
 // in flight per warp.  Twelve warps in one CTA per SM were as fast or slower
 // (a CTA's start is then hidden by no other) but for one sequence of 32768
 // tokens (22.6 against 24.7 us when it was compared), which cannot fill the
-// machine from clusters.  Now: 64 bf16 sequences of up to 2523 tokens 43.8 us
-// (4.24 TB/s), one of 32768 26.6 us, one of 512 13.5 us with the call.
+// machine from clusters.  Now, with the call and cold caches: 64 bf16 sequences
+// of up to 2523 tokens 43.7 us (4.25 TB/s), one of 32768 26.6 us, one of 512
+// 13.5 us.
 constexpr int kDWarps = 4;
 constexpr int kDThreads = kDWarps * 32;
 template <int HD>
@@ -579,8 +579,11 @@ cudaError_t launch_kv8_attend(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, 
     // of time, a tile's start about 30 of them.  The prompt kernel walks them once for 128 or 256 slots, one CTA per SM:
     // wave by wave a page takes 3 units, its start and end about 80 pages.  The wrong one is up
     // to 17 times slower (one f32 sequence of 16000 tokens, 64 slots, 8 heads: 104 us here, 275 there; 64 sequences of 2500:
-    // 780 and 286; of 8 slots: 115 and 266; one of 100 with 64 slots: 4.5 and 12.7).  Over 920 calls of both kernels the
-    // choice is 0.3 % from the better one on average and 23 % at most.
+    // 780 and 286; of 8 slots: 115 and 266; one of 100 with 64 slots: 4.5 and 12.7).  Over 920 calls of both kernels with
+    // tables as wide as the longest sequence the choice is 0.3 % from the better one on average and 23 % at most.  Without
+    // a window the table's width stands for the lengths, which the host does not know: 64 bf16 sequences of 100 tokens
+    // take 9.0 us with a table of their width or 8 times that, 49 with one of 64 times, whose clusters find no pages; 8
+    // f32 ones of 3000 14.5 and 28.7; a prompt of 60 f32 rows 7.4 and 24.7.
     const long long prompt_slots = kv8_prompt_slots(a.q.type);
     const long long waves = (tiles_of(prompt_slots) * groups + d.sms - 1) / d.sms;
     if (tiles > 65535 || (double)units * (pages + 30) > 3.0 * d.sms * waves * (pages_of(prompt_slots) + 80)) {
@@ -592,7 +595,7 @@ cudaError_t launch_kv8_attend(const Kv8 &c, const Kv8Rows &r, const Kv8Attn &a, 
     // where the machine is full (64 sequences of up to 2523 tokens: 46 us whole, 43.6 halved, 48 in thirds; 8 of up
     // to 6095: 20.6 in fourths, 18.9 in sixths, 24.2 in sevenths; 16 of 4000 visible ones: 18.4 in thirds, 16.4 in
     // fourths, 22.5 in sixths).  With SMs left over, down to a pair of pages per warp (one sequence of 512 tokens:
-    // 6.7 us in the kernel whole, 5.1 in pieces).
+    // 6.7 us in the kernel whole, 5.1 in pieces, replayed one after another).
     long long want = (pages + 32) / 64;
     if (units * want < d.sms) want = std::min(d.sms / units, pages / (2 * kDWarps));
     const int cs = (int)std::min<long long>(std::max<long long>(want, 1), kMaxCluster);

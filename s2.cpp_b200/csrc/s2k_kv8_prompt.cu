@@ -36,10 +36,12 @@
 // half of the dimensions by each group, with the step's own largest weight and
 // product as its references.
 //
-// Measured: 2 x 4096 bf16 rows, 32 / 8 heads of 128: 319 us, 613 TFLOP/s; 8191
-// f16 rows under a window of 1000, 16 / 4 heads of 64: 130 us, 256 TFLOP/s; 1024
-// f32 rows, 32 / 8 heads of 128: 50 us, 171 TFLOP/s.  A step of both groups takes
-// ~4800 cycles: a group's scores, weights and products wait for one another.
+// Measured: 2 x 4096 bf16 rows, 32 / 8 heads of 128: 322 us, 607 TFLOP/s; 8191
+// f16 rows under a window of 1000, 16 / 4 heads of 64: 133 us, 248 TFLOP/s; 1024
+// f32 rows, 32 / 8 heads of 128: 52 us, 166 TFLOP/s.  With weights relative to the
+// largest scale these took 318, 129 and 50.  A step of both groups takes ~4800
+// cycles (stamped in a build at 312 us): a group's scores, weights and products
+// wait for one another.
 #include "s2k_common.cuh"
 #include "s2k_kv8.h"
 #include "s2k_tc.cuh"
