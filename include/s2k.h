@@ -650,8 +650,7 @@ S2K_API s2k_status s2k_kv8_read(const s2k_kv8 *c, int32_t layer, const s2k_kv8_r
  * Sums and softmax statistics are f32 or exacter.  Rounded on the way are
  *   in calls of few rows: queries to 2^-30 of their row's largest element, and
  *     weights * value scales to a fraction of the largest of 32 keys, 2^-30, or
- *     2^-16 for 16-bit rows of sequences with more than 4 (row, query head)
- *     pairs per kv head;
+ *     2^-16 for 16-bit rows where max_rows * n_heads / n_kv_heads is above 4;
  *   in calls of many rows: weights * value scales to f16 (f32 rows: to 22 bits,
  *     and the queries too).
  * Which of the two a call is, and how its work is split, follows from n_seqs,
